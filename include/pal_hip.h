@@ -142,6 +142,32 @@ int pal_rope_fill_kv_pages(const void* new_keys, const void* new_values, int src
                            int num_q_heads, int q_out_dtype, void* stream);
 
 /*
+ * pal_rope_fill_kv_pages with rotary positions of several axes (time, height
+ * and width of image and video tokens), apart from the write positions.  No
+ * reference counterpart.  rotary_positions: device [num_axes, num_tokens],
+ * num_axes 1 .. 4; sections: HOST array of num_axes frequency counts that sum
+ * to rotary_dim / 2.  Frequency f of token t turns by the angle of row
+ * rotary_positions[a(f), t] of cos_sin_cache, where a(f) is
+ *   interleaved 0: the axis whose section holds f (the first sections[0]
+ *     frequencies axis 0, the next sections[1] axis 1, ...);
+ *   interleaved 1: f mod num_axes while f < num_axes * sections of that axis,
+ *     otherwise axis 0 (axis a > 0 has at most the frequencies a, a + num_axes,
+ *     ... below rotary_dim / 2).
+ * Everything else is as there: K is rotated, cast and scattered by
+ * write_positions, V cast and scattered, queries rotated and cast.  Tokens with
+ * a position that has no row in the table are not written to the pools; their
+ * queries are cast without rotation.
+ */
+int pal_mrope_fill_kv_pages(const void* new_keys, const void* new_values, int src_dtype, void* k_pool, void* v_pool,
+                            int kv_dtype, const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                            const int32_t* write_positions, const uint32_t* query_to_seq_map, int64_t num_tokens,
+                            int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages, int64_t num_seqs,
+                            int64_t page_table_width, const int32_t* rotary_positions, int num_axes,
+                            const int* sections, int interleaved, const float* cos_sin_cache, int64_t cos_sin_rows,
+                            int rotary_dim, int rope_style, const void* queries, void* queries_out, int num_q_heads,
+                            int q_out_dtype, void* stream);
+
+/*
  * Workspace bytes pal_paged_attention_decode needs for these shapes on the
  * current device (0 for unsupported arguments or when no device is present).
  * The workspace holds a scan of the sequence lengths, a work-claim counter

@@ -55,6 +55,7 @@ PAL_DEBUG_FLAGS_DEFINE(decode_debug_flags)
 
 }  // namespace pal
 
+#include "decode_plan.h"
 #include "prefill_half_tile.h"  // the fused kernels' prefill tiles (and prefill_tile.h)
 
 namespace pal {
@@ -82,105 +83,6 @@ constexpr int kGroupThreads = kWorkersPerGroup * kWave;
 constexpr int kPlanThreads = 1024;
 constexpr int kInlinePlanSeqs = 1024;  // largest batch scanned into LDS by each workgroup
 constexpr int64_t kMergeGroups = 2048;  // merge grid (at most): workgroups stride over the list
-
-struct Item {
-  int64_t row;  // query / output row
-  int64_t seq;  // page-table row
-  int64_t len;  // visible keys, clamped to [0, W * TPP]
-  bool skip;    // row mode: a row of a multi-row run (not ours to write)
-};
-
-__device__ __forceinline__ Item item_at(const DecodeParams& p, int64_t i, int tpp) {
-  Item it;
-  int64_t len;
-  it.row = i;
-  it.skip = false;
-  if (p.q2seq) {
-    const uint32_t sq = p.q2seq[i];
-    it.skip = (i > 0 && p.q2seq[i - 1] == sq) || (i + 1 < p.num_seqs && p.q2seq[i + 1] == sq);
-    if (sq < p.num_pt_rows && !it.skip) {
-      it.seq = sq;
-      len = p.seq_lens[sq];
-      const int64_t off = p.q_offset[i];
-      len = off < len ? off : len;
-    } else {  // no such sequence, or a prefill row: nothing to attend to here
-      it.seq = 0;
-      len = 0;
-    }
-  } else {
-    it.seq = i;
-    len = p.seq_lens[i];
-  }
-  const int64_t max_tokens = p.page_table_width * tpp;
-  PAL_DEBUG_FLAG(len > max_tokens, kDebugLength);
-  it.len = len < 0 ? 0 : (len > max_tokens ? max_tokens : len);
-  return it;
-}
-
-// The fixed cut of the global block list into virtual workers.
-// Equal shares: [0, T) split evenly over nws = min(resident workers, T)
-// virtual workers (none empty).  Fixed chunks: nc chunks of `chunk` blocks,
-// virtual ids nws + k with nws = 0.  (A dynamically claimed tail of chunks
-// after static shares measured much slower: each claimed range restarts the
-// load pipeline and writes its own partials.)
-struct Sched {
-  int64_t total;  // T: blocks of all segments
-  int64_t ts;     // static region [0, ts), split evenly over nws workers
-  int64_t nws;    // static virtual workers
-  int64_t chunk;  // blocks per chunk
-  int64_t nc;     // chunks covering [ts, total); virtual ids nws .. nws + nc - 1
-};
-
-__device__ __forceinline__ Sched make_sched(int64_t total, int64_t nw, int tokens_per_worker) {
-  Sched sc;
-  sc.total = total;
-  if (tokens_per_worker <= 0) {  // equal shares: no division on the start-up path
-    sc.ts = total;
-    sc.chunk = 1;
-    sc.nws = total < nw ? total : nw;
-    sc.nc = 0;
-    return sc;
-  }
-  // fixed-size chunks (the reference's CHUNK_SIZE mode)
-  sc.ts = 0;
-  sc.chunk = tokens_per_worker / 16 > 0 ? tokens_per_worker / 16 : 1;
-  sc.nws = 0;
-  sc.nc = (total + sc.chunk - 1) / sc.chunk;
-  return sc;
-}
-
-// First global block of virtual worker v (v in [0, nws + nc]); every virtual
-// worker owns at least one block.
-__device__ __forceinline__ int64_t vstart(const Sched& sc, int64_t v) {
-  if (v <= sc.nws) return sc.nws > 0 ? (v * sc.ts) / sc.nws : 0;
-  const int64_t b = sc.ts + (v - sc.nws) * sc.chunk;
-  return b < sc.total ? b : sc.total;
-}
-
-// Virtual worker whose range holds global block b.
-__device__ __forceinline__ int64_t vworker_of(const Sched& sc, int64_t b) {
-  if (b < sc.ts) return ((b + 1) * sc.nws + sc.ts - 1) / sc.ts - 1;
-  return sc.nws + (b - sc.ts) / sc.chunk;
-}
-
-// Zeros for every head of an empty item (no visible key).  Run by the
-// planner's thread that finds the item; such items are rare.
-template <int HD>
-__device__ __forceinline__ void zero_item_output(const DecodeParams& p, int64_t row) {
-  u32x2* o = reinterpret_cast<u32x2*>(p.out + row * p.num_q_heads * HD);  // out is 8-byte aligned
-  const int64_t n = static_cast<int64_t>(p.num_q_heads) * HD / 4;
-  for (int64_t i = 0; i < n; ++i) o[i] = u32x2{0u, 0u};
-}
-
-// Sequence holding global block b: the largest s with cum[s] <= b.
-__device__ __forceinline__ int64_t locate_seq(const int64_t* cum, int64_t num_seqs, int64_t b) {
-  int64_t lo = 0, hi = num_seqs - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (cum[mid] <= b) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
 
 // Scan for batches larger than kInlinePlanSeqs: cum[s] = first global block of
 // sequence s (all of its segments), cum[S] = hdr[0] = T.  Each thread takes

@@ -34,6 +34,12 @@
 //    GPT-J style pairs (2f, 2f + 1).  The products are rounded as written
 //    (no fused multiply-add), so results are bit-exact against a scalar fp32
 //    restatement.
+//  * RoPE over several axes (image and video tokens): frequency f turns by the
+//    token's position along axis a(f), and the positions are an input of their
+//    own, apart from the write positions.  A workgroup gathers its window's
+//    rows, each frequency's cos and sin from its axis' table row, into LDS once;
+//    from there on a token has one row, as above.  Query workgroups take several
+//    heads of their window, which share the gathered rows.
 //  * fp8: q = x / scale[page, h], held to [-448, 448] (NaN stays NaN), then
 //    rounded to nearest even e4m3.
 // Tokens whose destination falls outside the page table or the pool are
@@ -291,15 +297,146 @@ __device__ __forceinline__ void unit_chunks(const FillParams& p, int style, int 
 }
 
 // Rotates the unit's chunk(s) in place (x: chunk c0, y: chunk c1 of a NeoX
-// pair) with row `pos` of the table, when rotate.
-__device__ __forceinline__ void rotate_unit(const FillParams& p, int style, int c0, int c1, int pos, bool rotate,
+// pair) by the cos/sin row cs, when rotate.
+__device__ __forceinline__ void rotate_unit(const FillParams& p, int style, int c0, int c1, const float* cs, bool rotate,
                                             float (&x)[8], float (&y)[8]) {
   if (!rotate || style == 0 || 8 * c0 >= p.rotary_dim) return;
-  const float* cs = p.cos_sin + static_cast<int64_t>(pos) * p.rotary_dim;
   const bool neox = style == 1;
   if (neox && c1 < 0) return;
   rope_unit(x, y, cs, neox ? 8 * c0 : 4 * c0, p.rotary_dim / 2, neox);
 }
+
+// What a fill kernel is compiled for: the plain fill, RoPE by the write
+// positions, RoPE by positions of several axes.
+constexpr int kPlain = 0, kRope = 1, kRopeAxes = 2;
+constexpr int kAxesQueryHeads = 4;  // query heads of a workgroup (kRopeAxes)
+
+// Axis of frequency f: the section that holds it or, with interleaved axes,
+// f mod axes while that axis has frequencies left, and then axis 0.
+__device__ __forceinline__ int rope_axis(const FillParams& p, int f) {
+  if (p.rope_interleaved) {
+    const int a = f % p.rope_axes;
+    const int n = a == 0 ? 0 : (a == 1 ? p.rope_section_end[1] - p.rope_section_end[0]
+                                       : (a == 2 ? p.rope_section_end[2] - p.rope_section_end[1]
+                                                 : p.rope_section_end[3] - p.rope_section_end[2]));
+    return f < p.rope_axes * n ? a : 0;
+  }
+  return (f >= p.rope_section_end[0]) + (f >= p.rope_section_end[1]) + (f >= p.rope_section_end[2]);
+}
+// Do all positions of token t have a row in the table?
+__device__ __forceinline__ bool rope_axes_ok(const FillParams& p, int64_t t) {
+  bool ok = true;
+  for (int a = 0; a < p.rope_axes; ++a) {
+    const int pos = p.rope_pos[a * p.num_tokens + t];
+    ok = ok && pos >= 0 && pos < p.cos_sin_rows;
+  }
+  return ok;
+}
+// Gathers the cos/sin rows of the window's tokens into LDS (a position without a
+// row takes row 0: such a token is not rotated).
+__device__ __forceinline__ void gather_rope_rows(const FillParams& p, int64_t t0, int nwin, float* rows) {
+  const int half = p.rotary_dim / 2;
+  for (int it = threadIdx.x; it < nwin * half; it += kThreads) {
+    const int i = it / half;
+    const int f = it - i * half;
+    const int pos = p.rope_pos[rope_axis(p, f) * p.num_tokens + t0 + i];
+    const float* cs = p.cos_sin + (pos >= 0 && pos < p.cos_sin_rows ? static_cast<int64_t>(pos) * p.rotary_dim : 0);
+    rows[i * p.rotary_dim + f] = cs[f];
+    rows[i * p.rotary_dim + half + f] = cs[half + f];
+  }
+}
+
+// A 16-byte piece of a source row: 4 fp32 or 8 16-bit values.
+template <int SRC>
+constexpr int piece_values() { return SRC == kF32 ? 4 : 8; }
+template <int SRC>
+__device__ __forceinline__ void piece_to_f32(u32x4 w, float (&x)[piece_values<SRC>()]) {
+#pragma unroll
+  for (int e = 0; e < piece_values<SRC>(); ++e) {
+    if constexpr (SRC == kF32) x[e] = __uint_as_float(w[e]);
+    else x[e] = Dt<SRC>::to_f32(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+  }
+}
+template <int SRC>
+__device__ __forceinline__ void store_query_piece(const FillParams& p, int64_t elem, const float (&x)[piece_values<SRC>()]) {
+  constexpr int kVal = piece_values<SRC>();
+  uint32_t w[kVal / 2];
+#pragma unroll
+  for (int e = 0; e < kVal / 2; ++e)
+    w[e] = p.q_out_dtype == kBF16 ? Dt<kBF16>::pack2(x[2 * e], x[2 * e + 1]) : Dt<kF16>::pack2(x[2 * e], x[2 * e + 1]);
+  uint16_t* dst = static_cast<uint16_t*>(p.q_out) + elem;
+  if constexpr (SRC == kF32) __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2*>(dst));
+  else __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4*>(dst));
+}
+
+// kRopeAxes: rotates and casts query heads h0 .. h0 + nh - 1 of the window.  A
+// unit is a 16-byte piece of a head or, with NeoX rotation, a piece of the
+// rotated part's first half and its partner, so that no value crosses lanes.
+// Units run fastest, then heads: a wavefront reads whole lines.
+#pragma clang fp contract(off)
+template <int SRC, int kItems>
+__device__ __forceinline__ void rotate_queries_axes(const FillParams& p, int64_t t0, int nwin, int h0, int nh,
+                                                    const float* rows, const int* row_ok) {
+  constexpr int kVal = piece_values<SRC>();
+  constexpr int kSrcBytes = SRC == kF32 ? 4 : 2;
+  const int hd = p.head_dim, rot = p.rotary_dim, half = rot / 2;
+  const bool neox = p.rope_style == 1;
+  const int pairs = neox ? half / kVal : 0;
+  const int units = hd / kVal - pairs;
+  const int n_items = nwin * nh * units;
+  const int64_t q_row = static_cast<int64_t>(p.num_q_heads) * hd;
+  // element offset of unit u's first (and partner) piece in its head
+  auto dim0 = [&](int u) { return u < pairs ? kVal * u : kVal * (u + pairs); };
+#pragma unroll 1
+  for (int base = 0; base < n_items; base += kItems * kThreads) {
+    u32x4 a[kItems], b[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int it = base + static_cast<int>(threadIdx.x) + k * kThreads;
+      if (it < n_items) {
+        const int th = it / units, u = it - th * units;
+        const int i = th / nh;
+        const int64_t elem = (t0 + i) * q_row + static_cast<int64_t>(h0 + th - i * nh) * hd + dim0(u);
+        const uint8_t* src = static_cast<const uint8_t*>(p.q_in) + elem * kSrcBytes;
+        a[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src));
+        if (u < pairs) b[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + half * kSrcBytes));
+      }
+    }
+    if (base == 0) __syncthreads();  // the gathered rows are complete
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int it = base + static_cast<int>(threadIdx.x) + k * kThreads;
+      if (it >= n_items) continue;
+      const int th = it / units, u = it - th * units;
+      const int i = th / nh;
+      const int64_t elem = (t0 + i) * q_row + static_cast<int64_t>(h0 + th - i * nh) * hd + dim0(u);
+      const float* cs = rows + i * rot;
+      float x[kVal], y[kVal], xo[kVal], yo[kVal];
+      piece_to_f32<SRC>(a[k], x);
+#pragma unroll
+      for (int e = 0; e < kVal; ++e) xo[e] = x[e];
+      if (u < pairs) {
+        piece_to_f32<SRC>(b[k], y);
+#pragma unroll
+        for (int e = 0; e < kVal; ++e) {
+          const float c = cs[kVal * u + e], s = cs[half + kVal * u + e];
+          xo[e] = row_ok[i] ? x[e] * c - y[e] * s : x[e];
+          yo[e] = row_ok[i] ? y[e] * c + x[e] * s : y[e];
+        }
+        store_query_piece<SRC>(p, elem + half, yo);
+      } else if (!neox && kVal * u < rot && row_ok[i]) {
+#pragma unroll
+        for (int e = 0; e < kVal / 2; ++e) {
+          const float c = cs[kVal * u / 2 + e], s = cs[half + kVal * u / 2 + e];
+          xo[2 * e] = x[2 * e] * c - x[2 * e + 1] * s;
+          xo[2 * e + 1] = x[2 * e + 1] * c + x[2 * e] * s;
+        }
+      }
+      store_query_piece<SRC>(p, elem, xo);
+    }
+  }
+}
+#pragma clang fp contract(on)
 
 // Workgroup (w, y) of the grid: y < Hkv moves K and V of kv head y for the
 // window of WIN new tokens w * WIN ..; y >= Hkv (rope with queries only)
@@ -312,14 +449,17 @@ __device__ __forceinline__ void rotate_unit(const FillParams& p, int style, int 
 // from registers.  Run tokens' rows go through LDS, and each run is then
 // written in whole lines: K stripe q of its 8 slots (8 x 16 contiguous
 // bytes) and V row d of its 8 slots, the two runs of one page side by side
-// in neighbouring lanes.  ROPE false: the plain fill (no rotation, no
-// queries), compiled without the rotation code.
-template <int SRC, int DST, int WIN, int MAXC, bool ROPE>
+// in neighbouring lanes.  kMode kPlain: the plain fill (no rotation, no
+// queries), compiled without the rotation code.  kRopeAxes: y >= Hkv takes
+// kAxesQueryHeads query heads from (y - Hkv) * kAxesQueryHeads on.
+template <int SRC, int DST, int WIN, int MAXC, int kMode>
 __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParams p) {
   constexpr int kItems = (WIN * MAXC + kThreads - 1) / kThreads;  // source chunks per thread, at most
   constexpr int EB = elem_bytes<DST>();
   static_assert(WIN <= kWave, "the first wavefront classifies the window");
-  // dynamic LDS: the run tokens' K rows, then their V rows, [2][WIN][HD * EB + kRowPad] bytes
+  constexpr bool ROPE = kMode != kPlain;
+  // dynamic LDS: the run tokens' K rows, then their V rows, [2][WIN][HD * EB + kRowPad] bytes; kRopeAxes: then
+  // the tokens' cos/sin rows, [WIN][rotary_dim] fp32
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn_lds[];
   __shared__ uint32_t page_lds[WIN];  // destination page of each window token
   __shared__ int slot_lds[WIN];       // its slot, or -1: no valid destination
@@ -336,8 +476,18 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
   const int nwin = static_cast<int>(min(static_cast<int64_t>(WIN), p.num_tokens - t0));
   const int style = ROPE ? p.rope_style : 0;
   const int units = k_units(p, style);
+  float* rope_rows = reinterpret_cast<float*>(dyn_lds + 2 * WIN * (hd * EB + kRowPad));
+  if constexpr (kMode == kRopeAxes) {
+    if (static_cast<int>(blockIdx.y) >= p.num_kv_heads) {
+      const int h0 = (static_cast<int>(blockIdx.y) - p.num_kv_heads) * kAxesQueryHeads;
+      if (tid < nwin) kind_lds[tid] = rope_axes_ok(p, t0 + tid);
+      gather_rope_rows(p, t0, nwin, rope_rows);
+      rotate_queries_axes<SRC, 4>(p, t0, nwin, h0, min(kAxesQueryHeads, p.num_q_heads - h0), rope_rows, kind_lds);
+      return;
+    }
+  }
 
-  if (ROPE && static_cast<int>(blockIdx.y) >= p.num_kv_heads) {
+  if (kMode == kRope && static_cast<int>(blockIdx.y) >= p.num_kv_heads) {
     // ---- queries: rotate and cast head qh of the window's rows (a row is
     // contiguous in and out, so units run fastest: whole lines per wave)
     const int qh = blockIdx.y - p.num_kv_heads;
@@ -424,7 +574,8 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
       float x[8], y[8];
       rx[k].to_f32(x);
       if (c1 >= 0) ry[k].to_f32(y);
-      rotate_unit(p, style, c0, c1, pos[k], pos[k] >= 0 && pos[k] < p.cos_sin_rows, x, y);
+      const bool has_row = pos[k] >= 0 && pos[k] < p.cos_sin_rows;
+      rotate_unit(p, style, c0, c1, p.cos_sin + (has_row ? static_cast<int64_t>(pos[k]) * p.rotary_dim : 0), has_row, x, y);
       uint16_t* qo = static_cast<uint16_t*>(p.q_out) + (t0 + i) * q_row + static_cast<int64_t>(qh) * hd;
       if (p.q_out_dtype == kBF16) {
         *reinterpret_cast<u32x4*>(qo + 8 * c0) = Store8<kBF16>::pack(x, 1.f);
@@ -501,7 +652,7 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
       const uint32_t seq = p.q2seq[t];
       pos = p.write_pos[t];
       if (seq < p.num_seqs && pos >= 0 && pos / tpp < p.page_table_width &&
-          (style == 0 || pos < p.cos_sin_rows)) {
+          (kMode == kRopeAxes ? rope_axes_ok(p, t) : style == 0 || pos < p.cos_sin_rows)) {
         const uint32_t page = p.page_table[static_cast<int64_t>(seq) * p.page_table_width + pos / tpp];
         if (page < p.num_pages) {
           dpage = page;
@@ -520,7 +671,13 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
     ks_lds[tid] = ks;
     vs_lds[tid] = vs;
   }
+  if constexpr (kMode == kRopeAxes) gather_rope_rows(p, t0, nwin, rope_rows);
   __syncthreads();
+  // the cos/sin row of window token i
+  auto rope_row = [&](int i) {
+    if constexpr (kMode == kRopeAxes) return static_cast<const float*>(rope_rows + i * p.rotary_dim);
+    else return p.cos_sin + static_cast<int64_t>(pos_lds[i]) * p.rotary_dim;
+  };
   if (tid < kWave) {
     // A full run: slots 8k..8k+7 of one page (pages of a multiple of 8
     // slots, so the run's pieces of K stripes and V rows are aligned)
@@ -564,8 +721,7 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[sd][e] = pk[k][sd][e];
         if (style != 0)
-          rope_piece_pair(x[0], x[1], p.cos_sin + static_cast<int64_t>(pos_lds[i]) * p.rotary_dim, j, style,
-                          p.rotary_dim, hd);
+          rope_piece_pair(x[0], x[1], rope_row(i), j, style, p.rotary_dim, hd);
         const bool single = kind_lds[i] == 1;
         const int64_t hb = (static_cast<int64_t>(page_lds[i]) * p.num_kv_heads + h) * head_block;
 #pragma unroll
@@ -609,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
           float x[8], y[8];
           kx[k].to_f32(x);
           if (c1 >= 0) ky[k].to_f32(y);
-          rotate_unit(p, style, c0, c1, pos_lds[i], true, x, y);
+          if constexpr (ROPE) rotate_unit(p, style, c0, c1, rope_row(i), true, x, y);
           a = Store8<DST>::pack(x, ks_lds[i]);
           if (c1 >= 0) b = Store8<DST>::pack(y, ks_lds[i]);
         }
@@ -755,9 +911,9 @@ __global__ __launch_bounds__(kTokensThreads) void fill_tokens_kernel(const FillP
   for (int e = 0; e < 8; ++e) vp[e * tpp] = static_cast<uint16_t>(vw[e >> 1] >> (16 * (e & 1)));
 }
 
-template <int SRC, int DST, int MAXC, bool ROPE>
+template <int SRC, int DST, int MAXC, int kMode>
 hipError_t launch_win(const FillParams& p, hipStream_t stream) {
-  if constexpr (!ROPE && SRC == DST && DST != kFP8) {
+  if constexpr (kMode == kPlain && SRC == DST && DST != kFP8) {
     if (p.num_tokens <= kSmallFillTokens) {
       const int64_t n = p.num_tokens * p.num_kv_heads * (p.head_dim / 8);
       hipLaunchKernelGGL(fill_tokens_kernel, dim3(static_cast<unsigned>((n + kTokensThreads - 1) / kTokensThreads)),
@@ -769,13 +925,15 @@ hipError_t launch_win(const FillParams& p, hipStream_t stream) {
   // still spreads over 4 x 2 Hkv workgroups; prefill batches: 32
   const int win = p.num_tokens >= 2048 ? kLargeWin : kSmallWin;
   const int64_t windows = (p.num_tokens + win - 1) / win;
-  const unsigned gy = p.num_kv_heads + (p.q_in ? p.num_q_heads : 0);
-  const size_t lds = 2 * static_cast<size_t>(win) * (p.head_dim * elem_bytes<DST>() + kRowPad);  // K and V rows
+  const int q_groups = kMode == kRopeAxes ? (p.num_q_heads + kAxesQueryHeads - 1) / kAxesQueryHeads : p.num_q_heads;
+  const unsigned gy = p.num_kv_heads + (p.q_in ? q_groups : 0);
+  size_t lds = 2 * static_cast<size_t>(win) * (p.head_dim * elem_bytes<DST>() + kRowPad);  // K and V rows
+  if (kMode == kRopeAxes) lds += static_cast<size_t>(win) * p.rotary_dim * sizeof(float);
   if (win == kLargeWin)
-    hipLaunchKernelGGL((fill_kv_pages_kernel<SRC, DST, kLargeWin, MAXC, ROPE>), dim3(static_cast<unsigned>(windows), gy),
+    hipLaunchKernelGGL((fill_kv_pages_kernel<SRC, DST, kLargeWin, MAXC, kMode>), dim3(static_cast<unsigned>(windows), gy),
                        dim3(kThreads), lds, stream, p);
   else
-    hipLaunchKernelGGL((fill_kv_pages_kernel<SRC, DST, kSmallWin, MAXC, ROPE>), dim3(static_cast<unsigned>(windows), gy),
+    hipLaunchKernelGGL((fill_kv_pages_kernel<SRC, DST, kSmallWin, MAXC, kMode>), dim3(static_cast<unsigned>(windows), gy),
                        dim3(kThreads), lds, stream, p);
   return hipGetLastError();
 }
@@ -783,11 +941,12 @@ hipError_t launch_win(const FillParams& p, hipStream_t stream) {
 template <int SRC, int DST>
 hipError_t launch_t(const FillParams& p, hipStream_t stream) {
   // per-thread item registers sized for the head dim: up to 128 or up to 256
-  const bool rope = p.rope_style != 0 || p.q_in != nullptr;
-  if (p.head_dim <= 128)
-    return rope ? launch_win<SRC, DST, 16, true>(p, stream) : launch_win<SRC, DST, 16, false>(p, stream);
-  return rope ? launch_win<SRC, DST, kMaxFillHeadDim / 8, true>(p, stream)
-              : launch_win<SRC, DST, kMaxFillHeadDim / 8, false>(p, stream);
+  constexpr int kWide = kMaxFillHeadDim / 8;
+  const bool wide = p.head_dim > 128;
+  if (p.rope_pos) return wide ? launch_win<SRC, DST, kWide, kRopeAxes>(p, stream) : launch_win<SRC, DST, 16, kRopeAxes>(p, stream);
+  if (p.rope_style != 0 || p.q_in != nullptr)
+    return wide ? launch_win<SRC, DST, kWide, kRope>(p, stream) : launch_win<SRC, DST, 16, kRope>(p, stream);
+  return wide ? launch_win<SRC, DST, kWide, kPlain>(p, stream) : launch_win<SRC, DST, 16, kPlain>(p, stream);
 }
 
 template <int SRC>

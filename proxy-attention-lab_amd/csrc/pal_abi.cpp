@@ -218,6 +218,11 @@ struct FillArgs {
   void* queries_out = nullptr;
   int num_q_heads = 0;
   int q_out_dtype = PAL_DTYPE_BFLOAT16;
+  bool axes = false;  // several-axes RoPE: the next four
+  const int32_t* rotary_positions = nullptr;
+  int num_axes = 0;
+  const int* sections = nullptr;
+  bool interleaved = false;
 };
 
 int fill_call(const char* op, const FillArgs& a, hipStream_t stream) {
@@ -241,11 +246,33 @@ int fill_call(const char* op, const FillArgs& a, hipStream_t stream) {
                 pal::kMaxFillHeadDim);
   if (a.rope_style < 0 || a.rope_style > 2)
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] rope_style %d not in {0 none, 1 neox, 2 gptj}", op, a.rope_style);
+  if (a.axes && a.rope_style == 0)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] rope_style must be 1 neox or 2 gptj", op);
+  int section_end[4] = {0, 0, 0, 0};
   if (a.rope_style != 0) {
     const int mult = a.rope_style == 1 ? 16 : 8;
     if (a.rotary_dim <= 0 || a.rotary_dim > a.head_dim || a.rotary_dim % mult != 0)
       return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] rotary_dim %d must be a positive multiple of %d up to head_dim %d",
                   op, a.rotary_dim, mult, a.head_dim);
+    if (a.axes) {
+      if (a.num_axes < 1 || a.num_axes > 4 || !a.sections)
+        return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] 1 to 4 axes with their sections, got %d", op, a.num_axes);
+      const int half = a.rotary_dim / 2;
+      int64_t sum = 0;
+      for (int i = 0; i < a.num_axes; ++i) {
+        if (a.sections[i] < 0) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] negative section", op);
+        sum += a.sections[i];
+        // the frequencies an interleaved axis past the first can have: a, a + axes, ...
+        if (a.interleaved && i > 0 && static_cast<int64_t>(a.sections[i]) > (half - i + a.num_axes - 1) / a.num_axes)
+          return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] interleaved section %d of axis %d has no room in %d frequencies", op,
+                      a.sections[i], i, half);
+        section_end[i] = static_cast<int>(sum < half ? sum : half);
+      }
+      for (int i = a.num_axes; i < 4; ++i) section_end[i] = half;
+      if (sum != half)
+        return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] sections sum to %lld, rotary_dim / 2 is %d", op,
+                    static_cast<long long>(sum), half);
+    }
     if (a.cos_sin_rows < 0 || (a.num_tokens > 0 && (!a.cos_sin || a.cos_sin_rows == 0)))
       return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] rope needs a cos/sin table", op);
   }
@@ -257,7 +284,7 @@ int fill_call(const char* op, const FillArgs& a, hipStream_t stream) {
   }
   if (a.num_tokens == 0) return ok();
   if (!a.new_keys || !a.new_values || !a.k_pool || !a.v_pool || !a.page_table || !a.write_positions ||
-      !a.query_to_seq_map || (fp8 && (!a.k_scales || !a.v_scales)))
+      !a.query_to_seq_map || (fp8 && (!a.k_scales || !a.v_scales)) || (a.axes && !a.rotary_positions))
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] null pointer argument", op);
   if (!aligned16(a.new_keys) || !aligned16(a.new_values) || !aligned16(a.k_pool) || !aligned16(a.v_pool) ||
       (a.queries && (!aligned16(a.queries) || !aligned16(a.queries_out))))
@@ -289,6 +316,10 @@ int fill_call(const char* op, const FillArgs& a, hipStream_t stream) {
   p.q_out_dtype = a.q_out_dtype;
   p.rope_style = a.rope_style;
   p.rotary_dim = a.rope_style != 0 ? a.rotary_dim : 0;
+  p.rope_pos = a.axes ? a.rotary_positions : nullptr;
+  p.rope_axes = a.num_axes;
+  for (int i = 0; i < 4; ++i) p.rope_section_end[i] = section_end[i];
+  p.rope_interleaved = a.interleaved;
   PAL_LOG("%s tokens=%lld Hkv=%d HD=%d TPP=%d src=%d kv=%d rope=%d/%d queries=%d pages=%lld stream=%p", op,
           static_cast<long long>(a.num_tokens), a.num_kv_heads, a.head_dim, a.tokens_per_page, a.src_dtype,
           a.kv_dtype, a.rope_style, p.rotary_dim, a.queries ? a.num_q_heads : 0, static_cast<long long>(a.num_pages),
@@ -690,6 +721,49 @@ int pal_rope_fill_kv_pages(const void* new_keys, const void* new_values, int src
   a.num_q_heads = num_q_heads;
   a.q_out_dtype = q_out_dtype;
   return fill_call("rope_fill_kv_pages", a, static_cast<hipStream_t>(stream));
+}
+
+int pal_mrope_fill_kv_pages(const void* new_keys, const void* new_values, int src_dtype, void* k_pool, void* v_pool,
+                            int kv_dtype, const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                            const int32_t* write_positions, const uint32_t* query_to_seq_map, int64_t num_tokens,
+                            int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages, int64_t num_seqs,
+                            int64_t page_table_width, const int32_t* rotary_positions, int num_axes,
+                            const int* sections, int interleaved, const float* cos_sin_cache, int64_t cos_sin_rows,
+                            int rotary_dim, int rope_style, const void* queries, void* queries_out, int num_q_heads,
+                            int q_out_dtype, void* stream) {
+  FillArgs a;
+  a.new_keys = new_keys;
+  a.new_values = new_values;
+  a.src_dtype = src_dtype;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.kv_dtype = kv_dtype;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.page_table = page_table;
+  a.write_positions = write_positions;
+  a.query_to_seq_map = query_to_seq_map;
+  a.num_tokens = num_tokens;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.tokens_per_page = tokens_per_page;
+  a.num_pages = num_pages;
+  a.num_seqs = num_seqs;
+  a.page_table_width = page_table_width;
+  a.cos_sin = cos_sin_cache;
+  a.cos_sin_rows = cos_sin_rows;
+  a.rotary_dim = rotary_dim;
+  a.rope_style = rope_style;
+  a.queries = queries;
+  a.queries_out = queries_out;
+  a.num_q_heads = num_q_heads;
+  a.q_out_dtype = q_out_dtype;
+  a.axes = true;
+  a.rotary_positions = rotary_positions;
+  a.num_axes = num_axes;
+  a.sections = sections;
+  a.interleaved = interleaved != 0;
+  return fill_call("mrope_fill_kv_pages", a, static_cast<hipStream_t>(stream));
 }
 
 size_t pal_paged_attention_decode_workspace_size(int dtype, int64_t num_seqs, int num_q_heads,

@@ -43,6 +43,12 @@ struct FillParams {
   int q_out_dtype;             // kF16, kBF16
   int rope_style;              // 0 none, 1 NeoX (rotate halves), 2 GPT-J (rotate pairs)
   int rotary_dim;
+  // several axes: frequency f turns by the position along axis a(f) (null: every
+  // frequency by write_pos)
+  const int32_t* rope_pos;     // [rope_axes, N]
+  int rope_axes;               // 1 .. 4
+  int rope_section_end[4];     // running sums of the axes' frequencies; rotary_dim / 2 past the last axis
+  bool rope_interleaved;       // a(f) = f mod rope_axes while that axis has frequencies left, else 0
 };
 
 hipError_t launch_fill_kv_pages(const FillParams& p, hipStream_t stream);

@@ -15,6 +15,7 @@ from proxy_attention_lab.layout import FP8_DTYPE
 from proxy_attention_lab.page_pool import PagePool
 from proxy_attention_lab.ops import (
     fill_kv_pages,
+    mrope_fill_kv_pages,
     paged_attention,
     paged_attention_decode,
     paged_attention_prefill,
@@ -31,6 +32,7 @@ __all__ = [
     "get_k_cache_stripe_size",
     "get_optimal_page_size",
     "get_v_cache_shape",
+    "mrope_fill_kv_pages",
     "paged_attention",
     "paged_attention_decode",
     "paged_attention_prefill",

@@ -58,6 +58,13 @@ _SIGNATURES = {
         + [_c_i64, _c_int, _c_int, _c_int, _c_i64, _c_i64, _c_i64]
         + [_c_void_p, _c_i64, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
     ),
+    "pal_mrope_fill_kv_pages": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int] + [_c_void_p] * 5
+        + [_c_i64, _c_int, _c_int, _c_int, _c_i64, _c_i64, _c_i64]
+        + [_c_void_p, _c_int, ctypes.POINTER(_c_int), _c_int]
+        + [_c_void_p, _c_i64, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p],
+    ),
     "pal_paged_attention_decode_workspace_size": (
         _c_size_t,
         [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int],

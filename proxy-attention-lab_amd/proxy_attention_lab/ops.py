@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import collections
 import contextlib
+import ctypes
 
 import torch
 
@@ -36,6 +37,7 @@ from .layout import (  # noqa: F401  (get_k_cache_stripe_size re-exported)
 __all__ = [
     "fill_kv_pages",
     "get_k_cache_stripe_size",
+    "mrope_fill_kv_pages",
     "rope_cos_sin_cache",
     "rope_fill_kv_pages",
     "paged_attention",
@@ -434,6 +436,31 @@ def rope_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000.0
     return t
 
 
+def _rope_args(op: str, device: torch.device, n: int, hd: int, pool_dtype: torch.dtype, src_dtype: torch.dtype,
+               cos_sin_cache, queries, rotary_dim, style, query_dtype):
+    """Validation shared by the RoPE fills; returns (rotary_dim, Hq, query
+    output dtype, its code)."""
+    if style not in _ROPE_STYLES:
+        raise ValueError(f"[{op}] style must be 'neox' or 'gptj', got {style!r}")
+    rot = hd if rotary_dim is None else int(rotary_dim)
+    _require_device("cos_sin_cache", cos_sin_cache, device)
+    if cos_sin_cache.dim() != 2 or int(cos_sin_cache.shape[1]) != rot or cos_sin_cache.dtype != torch.float32:
+        raise ValueError(f"[{op}] cos_sin_cache must be float32 [rows, {rot}]")
+    hq = 0
+    if queries is not None:
+        _require_device("queries", queries, device)
+        if queries.dtype != src_dtype or queries.dim() != 3 or int(queries.shape[0]) != n or \
+                int(queries.shape[2]) != hd:
+            raise ValueError(f"[{op}] queries must be [{n}, Hq, {hd}] in the dtype of new_keys")
+        hq = int(queries.shape[1])
+        if query_dtype is None:
+            query_dtype = pool_dtype if pool_dtype != FP8_DTYPE else torch.bfloat16
+        q_code = dtype_code(query_dtype)
+    else:
+        q_code = _lib.DTYPE_BFLOAT16
+    return rot, hq, query_dtype, q_code
+
+
 def rope_fill_kv_pages(
     new_keys: torch.Tensor,
     new_values: torch.Tensor,
@@ -474,25 +501,9 @@ def rope_fill_kv_pages(
     device, n, num_pages, hkv, hd, tpp, width, num_seqs, pool_code, src_code = _fill_common(
         op, new_keys, new_values, global_key_pool, global_value_pool, page_table, current_token_write_positions,
         query_to_seq_map, k_scales, v_scales)
-    if style not in _ROPE_STYLES:
-        raise ValueError(f"[{op}] style must be 'neox' or 'gptj', got {style!r}")
-    rot = hd if rotary_dim is None else int(rotary_dim)
-    _require_device("cos_sin_cache", cos_sin_cache, device)
-    if cos_sin_cache.dim() != 2 or int(cos_sin_cache.shape[1]) != rot or cos_sin_cache.dtype != torch.float32:
-        raise ValueError(f"[{op}] cos_sin_cache must be float32 [rows, {rot}]")
+    rot, hq, query_dtype, q_code = _rope_args(op, device, n, hd, global_key_pool.dtype, new_keys.dtype, cos_sin_cache,
+                                              queries, rotary_dim, style, query_dtype)
     q_out = None
-    hq = 0
-    if queries is not None:
-        _require_device("queries", queries, device)
-        if queries.dtype != new_keys.dtype or queries.dim() != 3 or int(queries.shape[0]) != n or \
-                int(queries.shape[2]) != hd:
-            raise ValueError(f"[{op}] queries must be [{n}, Hq, {hd}] in the dtype of new_keys")
-        hq = int(queries.shape[1])
-        if query_dtype is None:
-            query_dtype = global_key_pool.dtype if pool_code != _lib.DTYPE_FP8_E4M3 else torch.bfloat16
-        q_code = dtype_code(query_dtype)
-    else:
-        q_code = _lib.DTYPE_BFLOAT16
     sh, sh_current = _launch_stream(stream, device)
     with _on_stream(sh, device, sh_current):
         if queries is not None:
@@ -510,6 +521,84 @@ def rope_fill_kv_pages(
             _ptr(nk), _ptr(nv), src_code, _ptr(global_key_pool), _ptr(global_value_pool), pool_code,
             _ptr(k_scales), _ptr(v_scales), _ptr(pt), _ptr(pos), _ptr(q2s), n, hkv, hd, tpp, num_pages, num_seqs,
             width, _ptr(cs), int(cs.shape[0]), rot, _ROPE_STYLES[style], _ptr(qi), _ptr(q_out), hq, q_code, sh)
+    _lib.check(status)
+    return global_key_pool, global_value_pool, q_out
+
+
+def mrope_fill_kv_pages(
+    new_keys: torch.Tensor,
+    new_values: torch.Tensor,
+    global_key_pool: torch.Tensor,
+    global_value_pool: torch.Tensor,
+    page_table: torch.Tensor,
+    current_token_write_positions: torch.Tensor,
+    query_to_seq_map: torch.Tensor,
+    rotary_positions: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    sections,
+    stream=None,
+    *,
+    interleaved: bool = False,
+    queries: torch.Tensor | None = None,
+    rotary_dim: int | None = None,
+    style: str = "neox",
+    query_dtype: torch.dtype | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """rope_fill_kv_pages with rotary positions of several axes: the time,
+    height and width of image and video tokens (no reference counterpart).
+
+    rotary_positions: [A, N] integers, A = len(sections) axes (1 to 4), apart
+    from current_token_write_positions, which only say where a token goes in
+    the cache.  sections: the axes' numbers of frequencies, summing to
+    rotary_dim / 2.  Frequency f of token t turns by the angle of row
+    rotary_positions[a(f), t] of ``cos_sin_cache``: a(f) is the axis whose
+    section holds f or, with ``interleaved``, f mod A while f < A *
+    sections[f mod A] and axis 0 past that.  Text tokens have the same
+    position on every axis, and are rotated as by rope_fill_kv_pages.
+
+    The other arguments, the casts, the scatter (in place) and the result
+    (key_pool, value_pool, rotated queries or None) are rope_fill_kv_pages';
+    tokens with a position that has no row in the table are not written to the
+    pools, and their queries are cast unrotated.
+    """
+    op = "mrope_fill_kv_pages"
+    device, n, num_pages, hkv, hd, tpp, width, num_seqs, pool_code, src_code = _fill_common(
+        op, new_keys, new_values, global_key_pool, global_value_pool, page_table, current_token_write_positions,
+        query_to_seq_map, k_scales, v_scales)
+    rot, hq, query_dtype, q_code = _rope_args(op, device, n, hd, global_key_pool.dtype, new_keys.dtype, cos_sin_cache,
+                                              queries, rotary_dim, style, query_dtype)
+    sections = tuple(int(s) for s in sections)
+    axes = len(sections)
+    if not 1 <= axes <= 4 or min(sections) < 0 or 2 * sum(sections) != rot:
+        raise ValueError(f"[{op}] sections must be 1 to 4 counts that sum to rotary_dim / 2 = {rot / 2:g}, got {sections}")
+    if interleaved and any(s > (rot // 2 - a + axes - 1) // axes for a, s in enumerate(sections) if a):
+        raise ValueError(f"[{op}] interleaved sections {sections}: an axis past the first has at most every "
+                         f"{axes}th of {rot // 2} frequencies")
+    _require_device("rotary_positions", rotary_positions, device)
+    if tuple(rotary_positions.shape) != (axes, n):
+        raise ValueError(f"[{op}] rotary_positions must be [{axes}, {n}], got {tuple(rotary_positions.shape)}")
+    q_out = None
+    sh, sh_current = _launch_stream(stream, device)
+    with _on_stream(sh, device, sh_current):
+        if queries is not None:
+            q_out = torch.empty((n, hq, hd), dtype=query_dtype, device=device)
+        if n == 0:
+            return global_key_pool, global_value_pool, q_out
+        pt = _index_tensor("page_table", page_table, device)
+        pos = _index_tensor("current_token_write_positions", current_token_write_positions, device)
+        q2s = _index_tensor("query_to_seq_map", query_to_seq_map, device)
+        rp = _index_tensor("rotary_positions", rotary_positions, device)
+        nk = new_keys.contiguous()
+        nv = new_values.contiguous()
+        cs = cos_sin_cache.contiguous()
+        qi = queries.contiguous() if queries is not None else None
+        status = _lib.lib().pal_mrope_fill_kv_pages(
+            _ptr(nk), _ptr(nv), src_code, _ptr(global_key_pool), _ptr(global_value_pool), pool_code,
+            _ptr(k_scales), _ptr(v_scales), _ptr(pt), _ptr(pos), _ptr(q2s), n, hkv, hd, tpp, num_pages, num_seqs,
+            width, _ptr(rp), axes, (ctypes.c_int * axes)(*sections), int(bool(interleaved)), _ptr(cs),
+            int(cs.shape[0]), rot, _ROPE_STYLES[style], _ptr(qi), _ptr(q_out), hq, q_code, sh)
     _lib.check(status)
     return global_key_pool, global_value_pool, q_out
 
