@@ -339,6 +339,53 @@ int pal_paged_attention_fp8(const void* queries, const void* k_pool, const void*
                             size_t workspace_bytes, void* stream);
 
 /*
+ * Differential attention over the paged cache (no reference counterpart; rows,
+ * lengths and pages as pal_paged_attention_decode and pal_paged_attention,
+ * ops.py:42-84).  The pools are those of ordinary attention, read in pairs: kv
+ * heads 2j and 2j + 1 hold the two keys K1, K2 of kv pair j and the first and
+ * second half of its 2 head_dim wide value, so every fill and page operation
+ * serves them as they are.  Query heads 2i and 2i + 1 are the two maps q1, q2 of
+ * output head i, which reads kv pair i / (num_q_heads / num_kv_heads):
+ *   x = softmax(q1 K1^T / sqrt(head_dim)) V - lambdas[i] softmax(q2 K2^T / sqrt(head_dim)) V
+ *   y = out_scale * x                                       without norm_weight
+ *   y = out_scale * norm_weight * x / sqrt(mean(x^2) + norm_eps)
+ * lambdas: fp32 [num_q_heads / 2]; norm_weight: fp32 [2 head_dim], shared by the
+ * heads, or NULL.  out: [rows, num_q_heads / 2, 2 head_dim] in dtype.  Sums,
+ * softmax statistics and both maps' outputs are held in fp32 until y is rounded;
+ * the probabilities are rounded to dtype for their product with the values.
+ * Rows without a visible key are zeros.  num_kv_heads even; kv_dtype dtype or
+ * fp8 (with k_scales and v_scales); head_dim 32, 64, 96 or 128 (fp8: 64, 128);
+ * tokens_per_page 16 or 32.  All pointers but lambdas, the index arrays and the
+ * scales 16-byte aligned.  The workspace (256-byte aligned) needs no initial
+ * contents; calls that may overlap need separate ones.  Its size is the same
+ * for both entries (num_query_rows: the sequences of a decode call).
+ */
+size_t pal_paged_differential_attention_workspace_size(int dtype, int kv_dtype, int64_t num_query_rows,
+                                                       int num_q_heads, int num_kv_heads, int head_dim,
+                                                       int tokens_per_page);
+/* One query row per sequence, row s of sequence s (rows >= num_seqs ignored;
+ * out: [num_seqs, ...]), over tokens [0, sequence_lengths[s]). */
+int pal_paged_differential_attention_decode(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
+                                            const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                                            const int32_t* sequence_lengths, const float* lambdas,
+                                            const float* norm_weight, float norm_eps, float out_scale, void* out,
+                                            int dtype, int64_t num_query_rows, int64_t num_seqs, int num_q_heads,
+                                            int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages,
+                                            int64_t page_table_width, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+/* Chunks of new tokens and decode rows in one call: row r of sequence s =
+ * query_to_seq_map[r] sees tokens [0, min(sequence_lengths[s],
+ * query_token_offset[r])). */
+int pal_paged_differential_attention(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
+                                     const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                                     const int32_t* sequence_lengths, const uint32_t* query_to_seq_map,
+                                     const int32_t* query_token_offset, const float* lambdas,
+                                     const float* norm_weight, float norm_eps, float out_scale, void* out, int dtype,
+                                     int64_t num_query_rows, int64_t num_seqs, int num_q_heads, int num_kv_heads,
+                                     int head_dim, int tokens_per_page, int64_t num_pages, int64_t page_table_width,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Page-pool allocator and compaction.  No reference counterpart: the
  * reference takes page tables from its caller (ops.py:61-63,
  * paged_attention_decode_primitive.cpp:71-266 reads them as an input); this

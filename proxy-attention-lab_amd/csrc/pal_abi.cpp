@@ -595,6 +595,96 @@ int decode_call(const void* queries, const void* k_pool, const void* v_pool, con
                     "paged_attention_decode");
 }
 
+bool diff_head_dim_supported(int hd, bool kv8) { return hd == 64 || hd == 128 || (!kv8 && (hd == 32 || hd == 96)); }
+
+// The shapes of both differential attention entry points; returns PAL_OK or an error.
+int check_diff_dims(const char* op, int dtype, int kv_dtype, int num_q_heads, int num_kv_heads, int head_dim,
+                    int tokens_per_page, int64_t num_pages, int64_t page_table_width) {
+  const int st = check_attention_dims(op, dtype, num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages,
+                                      page_table_width);
+  if (st != PAL_OK) return st;
+  if (kv_dtype != dtype && kv_dtype != PAL_DTYPE_FP8_E4M3)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] pools must hold the queries' dtype or fp8 (dtype codes %d, %d)", op,
+                dtype, kv_dtype);
+  if (num_kv_heads % 2 != 0)
+    return fail(PAL_ERR_RUNTIME, "[%s] num_kv_heads must be even, two to a pair (%d)", op, num_kv_heads);
+  const bool kv8 = kv_dtype == PAL_DTYPE_FP8_E4M3;
+  if (!diff_head_dim_supported(head_dim, kv8))
+    return fail(PAL_ERR_RUNTIME, "[%s] no %skernel for head_dim %d (supported: %s)", op, kv8 ? "fp8 " : "", head_dim,
+                kv8 ? "64, 128" : "32, 64, 96, 128");
+  return PAL_OK;
+}
+
+size_t diff_workspace_size(int dtype, int kv_dtype, int64_t num_rows, int num_q_heads, int num_kv_heads, int head_dim,
+                           int tokens_per_page) {
+  if (num_rows <= 0 || num_rows > 0x7fffffffLL ||
+      check_diff_dims("paged_differential_attention", dtype, kv_dtype, num_q_heads, num_kv_heads, head_dim,
+                      tokens_per_page, 0, 0) != PAL_OK)
+    return 0;
+  return 256;
+}
+
+// Rows of sequences: row i of sequence i (decode: no map), or of query_to_seq_map[i].
+int diff_call(const char* op, bool mapped, const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
+              const float* k_scales, const float* v_scales, const uint32_t* page_table,
+              const int32_t* sequence_lengths, const uint32_t* query_to_seq_map, const int32_t* query_token_offset,
+              const float* lambdas, const float* norm_weight, float norm_eps, float out_scale, void* out, int dtype,
+              int64_t num_rows, int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+              int tokens_per_page, int64_t num_pages, int64_t page_table_width, void* workspace,
+              size_t workspace_bytes, hipStream_t stream) {
+  const int st = check_diff_dims(op, dtype, kv_dtype, num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages,
+                                 page_table_width);
+  if (st != PAL_OK) return st;
+  const bool kv8 = kv_dtype == PAL_DTYPE_FP8_E4M3;
+  if (kv8 != (k_scales != nullptr) || kv8 != (v_scales != nullptr))
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] k_scales and v_scales go with fp8 pools, both", op);
+  if (num_rows < 0 || num_seqs < 0) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] negative dimension", op);
+  if (num_rows > 0x7fffffffLL || num_seqs > 0x7fffffffLL || page_table_width > 0x7fffffffLL / tokens_per_page)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] problem too large for one call", op);
+  if (!(norm_eps >= 0.f)) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] norm_eps must not be negative", op);
+  if (num_rows == 0) return ok();
+  if (num_pages == 0) page_table_width = 0;  // no page to read: every row is empty
+  if (!queries || !sequence_lengths || !lambdas || !out || (num_pages > 0 && (!k_pool || !v_pool)) ||
+      (page_table_width > 0 && !page_table) || (mapped && (!query_to_seq_map || !query_token_offset)))
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] null pointer argument", op);
+  if (!aligned16(queries) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(norm_weight) || !aligned16(out))
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] queries, pools, norm_weight and out must be 16-byte aligned", op);
+  const size_t need = diff_workspace_size(dtype, kv_dtype, num_rows, num_q_heads, num_kv_heads, head_dim, tokens_per_page);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace of %zu bytes needed, %zu given", op, need, workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace must be 256-byte aligned", op);
+  pal::DiffParams p{};
+  p.q = static_cast<const uint16_t*>(queries);
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  p.page_table = page_table;
+  p.seq_lens = sequence_lengths;
+  p.out = static_cast<uint16_t*>(out);
+  p.q2seq = mapped ? query_to_seq_map : nullptr;
+  p.q_offset = mapped ? query_token_offset : nullptr;
+  p.num_pt_rows = num_seqs;
+  p.num_seqs = num_rows;
+  p.num_pages = num_pages;
+  p.page_table_width = page_table_width;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads / 2;
+  p.group = num_q_heads / num_kv_heads;
+  p.head_chunks = (p.group + 7) / 8;
+  p.hg_max = p.group < 8 ? p.group : 8;
+  p.scale_log2 = scale_log2_for(head_dim);
+  p.lambdas = lambdas;
+  p.norm_weight = norm_weight;
+  p.norm_eps = norm_eps;
+  p.out_scale = out_scale;
+  PAL_LOG("%s rows=%lld seqs=%lld Hq=%d Hkv=%d HD=%d TPP=%d dtype=%d kv=%d norm=%d stream=%p", op,
+          static_cast<long long>(num_rows), static_cast<long long>(num_seqs), num_q_heads, num_kv_heads, head_dim,
+          tokens_per_page, dtype, kv_dtype, norm_weight ? 1 : 0, static_cast<void*>(stream));
+  return hip_status(pal::launch_diff(p, dtype, head_dim, tokens_per_page, stream), op);
+}
+
 }  // namespace
 
 extern "C" {
@@ -877,6 +967,45 @@ int pal_paged_attention_fp8(const void* queries, const void* k_pool, const void*
                     static_cast<hipStream_t>(stream));
 }
 
+size_t pal_paged_differential_attention_workspace_size(int dtype, int kv_dtype, int64_t num_query_rows,
+                                                       int num_q_heads, int num_kv_heads, int head_dim,
+                                                       int tokens_per_page) {
+  return diff_workspace_size(dtype, kv_dtype, num_query_rows, num_q_heads, num_kv_heads, head_dim, tokens_per_page);
+}
+
+int pal_paged_differential_attention_decode(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
+                                            const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                                            const int32_t* sequence_lengths, const float* lambdas,
+                                            const float* norm_weight, float norm_eps, float out_scale, void* out,
+                                            int dtype, int64_t num_query_rows, int64_t num_seqs, int num_q_heads,
+                                            int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages,
+                                            int64_t page_table_width, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+  const char* op = "paged_differential_attention_decode";
+  if (num_query_rows < num_seqs)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] %lld query rows for %lld sequences", op,
+                static_cast<long long>(num_query_rows), static_cast<long long>(num_seqs));
+  return diff_call(op, false, queries, k_pool, v_pool, kv_dtype, k_scales, v_scales, page_table, sequence_lengths,
+                   nullptr, nullptr, lambdas, norm_weight, norm_eps, out_scale, out, dtype, num_seqs, num_seqs,
+                   num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages, page_table_width, workspace,
+                   workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int pal_paged_differential_attention(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
+                                     const float* k_scales, const float* v_scales, const uint32_t* page_table,
+                                     const int32_t* sequence_lengths, const uint32_t* query_to_seq_map,
+                                     const int32_t* query_token_offset, const float* lambdas,
+                                     const float* norm_weight, float norm_eps, float out_scale, void* out, int dtype,
+                                     int64_t num_query_rows, int64_t num_seqs, int num_q_heads, int num_kv_heads,
+                                     int head_dim, int tokens_per_page, int64_t num_pages, int64_t page_table_width,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return diff_call("paged_differential_attention", true, queries, k_pool, v_pool, kv_dtype, k_scales, v_scales,
+                   page_table, sequence_lengths, query_to_seq_map, query_token_offset, lambdas, norm_weight, norm_eps,
+                   out_scale, out, dtype, num_query_rows, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                   tokens_per_page, num_pages, page_table_width, workspace, workspace_bytes,
+                   static_cast<hipStream_t>(stream));
+}
+
 int pal_copy_pages(void* k_pool, void* v_pool, float* k_scales, float* v_scales, int64_t num_pages, int num_kv_heads,
                    int64_t page_bytes, const uint32_t* src, const uint32_t* dst, int64_t num_moves, void* stream) {
   const char* op = "copy_pages";
@@ -915,12 +1044,13 @@ int pal_remap_pages(uint32_t* page_table, int64_t num_entries, const uint32_t* r
 int pal_debug_flags(int reset, uint32_t* flags) {
   if (!flags) return fail(PAL_ERR_INVALID_ARGUMENT, "[debug_flags] null output");
 #ifdef PAL_DEBUG_CHECKS
-  uint32_t a = 0, b = 0, c = 0;
+  uint32_t a = 0, b = 0, c = 0, d = 0;
   hipError_t err = pal::decode_debug_flags(&a, reset != 0);
   if (err == hipSuccess) err = pal::prefill_debug_flags(&b, reset != 0);
   if (err == hipSuccess) err = pal::fill_debug_flags(&c, reset != 0);
+  if (err == hipSuccess) err = pal::diff_debug_flags(&d, reset != 0);
   if (err != hipSuccess) return hip_status(err, "debug_flags");
-  *flags = a | b | c;
+  *flags = a | b | c | d;
   return ok();
 #else
   (void)reset;

@@ -170,6 +170,22 @@ bool fused_shares_cu(int head_dim);
 hipError_t launch_fused(const DecodeParams& dp, const PrefillParams& pp, int dtype, int head_dim, int tokens_per_page,
                         hipStream_t stream);
 
+// Differential attention over the pools of ordinary attention: kv heads 2j and
+// 2j + 1 are the two keys of kv pair j and the two halves of its value (two
+// neighbouring (page, kv head) blocks), query heads 2i and 2i + 1 the two maps of
+// output head i.  The base's fields keep their meaning with num_kv_heads the
+// number of kv PAIRS, num_q_heads of query heads, group of output heads per kv
+// pair, head_chunks of groups of 8 of them, hg_max = min(group, 8).  Rows as
+// in DecodeParams (row mode: every row, see launch_diff).
+struct DiffParams : DecodeParams {
+  const float* lambdas;      // [Hq / 2]
+  const float* norm_weight;  // [2 HD], or null: no norm
+  float norm_eps;
+  float out_scale;
+};
+
+hipError_t launch_diff(const DiffParams& p, int dtype, int head_dim, int tokens_per_page, hipStream_t stream);
+
 // Page moves of a compaction: pages src[m] -> dst[m] of both pools (whole
 // pages, page_bytes each) and, for fp8 pools, their scale rows.  Sources and
 // destinations must be disjoint sets.
@@ -195,6 +211,7 @@ hipError_t launch_remap_pages(uint32_t* table, int64_t n, const uint32_t* remap,
 hipError_t decode_debug_flags(uint32_t* out, bool reset);
 hipError_t prefill_debug_flags(uint32_t* out, bool reset);
 hipError_t fill_debug_flags(uint32_t* out, bool reset);
+hipError_t diff_debug_flags(uint32_t* out, bool reset);
 
 // Scratch memory held by the library for pal_paged_attention_decode_noalloc:
 // kScratchBytes per device, in a file-scope device array (scratch.hip).

@@ -14,11 +14,14 @@ from proxy_attention_lab.layout import (
 from proxy_attention_lab.layout import FP8_DTYPE
 from proxy_attention_lab.page_pool import PagePool
 from proxy_attention_lab.ops import (
+    differential_lambda,
     fill_kv_pages,
     mrope_fill_kv_pages,
     paged_attention,
     paged_attention_decode,
     paged_attention_prefill,
+    paged_differential_attention,
+    paged_differential_attention_decode,
     release_workspaces,
     rope_cos_sin_cache,
     rope_fill_kv_pages,
@@ -27,6 +30,7 @@ from proxy_attention_lab.ops import (
 __version__ = "2025.06.4+gfx950"
 
 __all__ = [
+    "differential_lambda",
     "fill_kv_pages",
     "get_k_cache_shape",
     "get_k_cache_stripe_size",
@@ -36,6 +40,8 @@ __all__ = [
     "paged_attention",
     "paged_attention_decode",
     "paged_attention_prefill",
+    "paged_differential_attention",
+    "paged_differential_attention_decode",
     "release_workspaces",
     "rope_cos_sin_cache",
     "rope_fill_kv_pages",

@@ -34,6 +34,7 @@ _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
 _c_void_p = ctypes.c_void_p
 _c_size_t = ctypes.c_size_t
+_c_float = ctypes.c_float
 
 # name -> (restype, argtypes); must match include/pal_hip.h
 _SIGNATURES = {
@@ -116,6 +117,22 @@ _SIGNATURES = {
     "pal_paged_attention": (
         _c_int,
         [_c_void_p] * 8
+        + [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64]
+        + [_c_void_p, _c_size_t, _c_void_p],
+    ),
+    "pal_paged_differential_attention_workspace_size": (
+        _c_size_t,
+        [_c_int, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int],
+    ),
+    "pal_paged_differential_attention_decode": (
+        _c_int,
+        [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 6 + [_c_float, _c_float, _c_void_p]
+        + [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64]
+        + [_c_void_p, _c_size_t, _c_void_p],
+    ),
+    "pal_paged_differential_attention": (
+        _c_int,
+        [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 8 + [_c_float, _c_float, _c_void_p]
         + [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64]
         + [_c_void_p, _c_size_t, _c_void_p],
     ),

@@ -35,6 +35,7 @@ from .layout import (  # noqa: F401  (get_k_cache_stripe_size re-exported)
 )
 
 __all__ = [
+    "differential_lambda",
     "fill_kv_pages",
     "get_k_cache_stripe_size",
     "mrope_fill_kv_pages",
@@ -43,6 +44,8 @@ __all__ = [
     "paged_attention",
     "paged_attention_decode",
     "paged_attention_prefill",
+    "paged_differential_attention",
+    "paged_differential_attention_decode",
     "release_workspaces",
 ]
 
@@ -755,3 +758,156 @@ def paged_attention(
             )
     _lib.check(status)
     return out
+
+
+def differential_lambda(lambda_q1: torch.Tensor, lambda_k1: torch.Tensor, lambda_q2: torch.Tensor,
+                        lambda_k2: torch.Tensor, lambda_init: float, num_heads: int) -> torch.Tensor:
+    """The lambdas the differential attention operators read, from a layer's
+    learned vectors: exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) +
+    lambda_init, float32 [num_heads], computed in float64 and rounded once.
+    The vectors are [D] (one lambda for every head) or [num_heads, D].  A
+    program computes it once, when it loads the weights."""
+    vectors = (lambda_q1, lambda_k1, lambda_q2, lambda_k2)
+    for t in vectors:
+        if not isinstance(t, torch.Tensor) or not t.is_floating_point() or t.dim() not in (1, 2) or \
+                t.shape != lambda_q1.shape or (t.dim() == 2 and int(t.shape[0]) != num_heads):
+            raise ValueError(f"[differential_lambda] the four vectors must be floating [D] or [{num_heads}, D], alike")
+    q1, k1, q2, k2 = (t.detach().double() for t in vectors)
+    lam = torch.exp((q1 * k1).sum(-1)) - torch.exp((q2 * k2).sum(-1)) + float(lambda_init)
+    return lam.to(torch.float32).expand(num_heads).contiguous()
+
+
+def _on_device(device: torch.device):
+    """Context in which ``device`` is the current one (launches and workspace
+    sizes go by it)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _differential(op: str, queries, k_pool, v_pool, page_table, lengths, q2s, offsets, lambdas, stream, norm_weight,
+                  norm_eps, out_scale, k_scales, v_scales) -> torch.Tensor:
+    """Validation, allocation and launch shared by the differential attention
+    operators (q2s and offsets None: decode)."""
+    _require_device("queries", queries)
+    device = queries.device
+    code = dtype_code(queries.dtype)
+    num_pages, hkv, hd, tpp = _pools(op, k_pool, v_pool, device, queries.dtype)
+    ks, vs = _scales(op, k_pool, k_scales, v_scales, num_pages, hkv, device)
+    if queries.dim() != 3 or int(queries.shape[2]) != hd:
+        raise ValueError(f"[{op}] queries must be 3D [N, Hq, {hd}], got {tuple(queries.shape)}")
+    num_rows, hq = int(queries.shape[0]), int(queries.shape[1])
+    if hq == 0 or hq % 2 or hkv % 2:
+        raise ValueError(f"[{op}] query and kv heads come in pairs, got {hq} and {hkv}")
+    if page_table.dim() != 2:
+        raise ValueError(f"[{op}] page_table must be 2D [num_seqs, max_pages_per_seq]")
+    num_seqs, width = (int(x) for x in page_table.shape)
+    _require_device("sequence_lengths", lengths, device)
+    if lengths.numel() < num_seqs:
+        raise ValueError(f"[{op}] {lengths.numel()} sequence lengths for {num_seqs} sequences")
+    if q2s is not None and (q2s.numel() != num_rows or offsets.numel() != num_rows):
+        raise ValueError(f"[{op}] query_to_seq_map and query_token_offset need one entry per query row ({num_rows})")
+    _require_device("lambdas", lambdas, device)
+    if lambdas.dtype != torch.float32 or tuple(lambdas.shape) != (hq // 2,):
+        raise ValueError(f"[{op}] lambdas must be float32 [{hq // 2}], got {lambdas.dtype} {tuple(lambdas.shape)}")
+    if norm_weight is not None:
+        _require_device("norm_weight", norm_weight, device)
+        if norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (2 * hd,):
+            raise ValueError(f"[{op}] norm_weight must be float32 [{2 * hd}], got {norm_weight.dtype} "
+                             f"{tuple(norm_weight.shape)}")
+    rows = num_seqs if q2s is None else num_rows
+    L = _lib.lib()
+    kv_code = pool_dtype_code(k_pool.dtype)
+    with _on_device(device):
+        sh, sh_current = _launch_stream(stream, device)
+        with _on_stream(sh, device, sh_current):
+            pt = _index_tensor("page_table", page_table, device)
+            lens = _index_tensor("sequence_lengths", lengths, device)
+            index = () if q2s is None else (_index_tensor("query_to_seq_map", q2s, device),
+                                            _index_tensor("query_token_offset", offsets, device))
+            q, kp, vp, lam = queries.contiguous(), k_pool.contiguous(), v_pool.contiguous(), lambdas.contiguous()
+            w = None if norm_weight is None else norm_weight.contiguous()
+            if ks is not None:
+                ks, vs = ks.contiguous(), vs.contiguous()
+            out = torch.empty((rows, hq // 2, 2 * hd), dtype=queries.dtype, device=device)
+            # a workspace of the call's own (it needs no initial contents): calls captured
+            # into different graphs share nothing
+            nbytes = L.pal_paged_differential_attention_workspace_size(code, kv_code, rows, hq, hkv, hd, tpp)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+            entry = L.pal_paged_differential_attention_decode if q2s is None else L.pal_paged_differential_attention
+            status = entry(
+                _ptr(q), _ptr(kp), _ptr(vp), kv_code, _ptr(ks), _ptr(vs), _ptr(pt), _ptr(lens),
+                *(_ptr(t) for t in index), _ptr(lam), _ptr(w), float(norm_eps), float(out_scale), _ptr(out), code,
+                num_rows, num_seqs, hq, hkv, hd, tpp, num_pages, width, _ptr(ws), nbytes, sh)
+    _lib.check(status)
+    return out
+
+
+def paged_differential_attention_decode(
+    queries: torch.Tensor,
+    k_cache_pool: torch.Tensor,
+    v_cache_pool: torch.Tensor,
+    page_table: torch.Tensor,
+    sequence_lengths: torch.Tensor,
+    lambdas: torch.Tensor,
+    stream=None,
+    *,
+    norm_weight: torch.Tensor | None = None,
+    norm_eps: float = 1e-5,
+    out_scale: float = 1.0,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Differential attention of one query row per sequence over its paged
+    context (no reference counterpart; rows and pages as
+    paged_attention_decode, ops.py:42-84).
+
+    The pools are those of ordinary attention, read in pairs: kv heads 2j and
+    2j + 1 hold the two keys of kv pair j and the two halves of its value, so
+    fill_kv_pages, rope_fill_kv_pages, mrope_fill_kv_pages and PagePool serve
+    them as they are.  queries: [N, Hq, HD], heads 2i and 2i + 1 the two maps
+    q1, q2 of output head i, which reads kv pair i // (Hq // Hkv):
+
+      x = (softmax(q1 K1^T / sqrt(HD)) - lambdas[i] softmax(q2 K2^T / sqrt(HD))) [V1 V2]
+      y = out_scale * x, or with norm_weight
+      y = out_scale * norm_weight * x / sqrt(mean(x^2) + norm_eps)
+
+    lambdas: float32 [Hq/2] (see differential_lambda); norm_weight: float32
+    [2 HD], shared by the heads; out_scale is usually 1 - lambda_init.
+    Returns [S, Hq/2, 2 HD] in the query dtype; a sequence without keys gives
+    zeros.  Hq and Hkv even, HD 32, 64, 96 or 128 (fp8 pools: 64, 128), pages of
+    16 or 32 tokens.
+    """
+    return _differential("paged_differential_attention_decode", queries, k_cache_pool, v_cache_pool, page_table,
+                         sequence_lengths, None, None, lambdas, stream, norm_weight, norm_eps, out_scale, k_scales,
+                         v_scales)
+
+
+def paged_differential_attention(
+    queries: torch.Tensor,
+    k_cache_pool: torch.Tensor,
+    v_cache_pool: torch.Tensor,
+    page_table: torch.Tensor,
+    sequence_lengths: torch.Tensor,
+    query_to_seq_map: torch.Tensor,
+    query_token_offset: torch.Tensor,
+    lambdas: torch.Tensor,
+    stream=None,
+    *,
+    norm_weight: torch.Tensor | None = None,
+    norm_eps: float = 1e-5,
+    out_scale: float = 1.0,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Differential attention of chunks of new tokens and decode rows in one
+    call: paged_attention's rows (row r of sequence s = query_to_seq_map[r] sees
+    tokens [0, min(sequence_lengths[s], query_token_offset[r])) of s's pages)
+    with paged_differential_attention_decode's heads.  Returns [R, Hq/2, 2 HD];
+    rows that see no token, or name no sequence, are zero."""
+    op = "paged_differential_attention"
+    _require_device("queries", queries)
+    for name, t in (("query_to_seq_map", query_to_seq_map), ("query_token_offset", query_token_offset)):
+        _require_device(name, t, queries.device)
+    return _differential(op, queries, k_cache_pool, v_cache_pool, page_table, sequence_lengths, query_to_seq_map,
+                         query_token_offset, lambdas, stream, norm_weight, norm_eps, out_scale, k_scales, v_scales)
