@@ -80,56 +80,7 @@ __device__ __forceinline__ T page_load(const T* p) {
   else return __builtin_nontemporal_load(p);
 }
 constexpr int kGroupThreads = kWorkersPerGroup * kWave;
-constexpr int kPlanThreads = 1024;
-constexpr int kInlinePlanSeqs = 1024;  // largest batch scanned into LDS by each workgroup
 constexpr int64_t kMergeGroups = 2048;  // merge grid (at most): workgroups stride over the list
-
-// Scan for batches larger than kInlinePlanSeqs: cum[s] = first global block of
-// sequence s (all of its segments), cum[S] = hdr[0] = T.  Each thread takes
-// kPlanPer consecutive items per pass, so their length loads go out together;
-// it also writes the zeros of an empty item.
-constexpr int kPlanPer = 16;
-
-template <int HD, int TPP>
-__global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const DecodeParams p) {
-  __shared__ int64_t wave_sums[kPlanThreads / kWave];
-  __shared__ int64_t carry_sh;
-  const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
-  const int tid = threadIdx.x;
-  int64_t carry = 0;
-  const int64_t n = p.num_seqs;
-  for (int64_t base = 0; base < n; base += static_cast<int64_t>(kPlanThreads) * kPlanPer) {
-    int64_t vals[kPlanPer];
-    int64_t tsum = 0;
-#pragma unroll
-    for (int k = 0; k < kPlanPer; ++k) {
-      const int64_t s = base + static_cast<int64_t>(tid) * kPlanPer + k;
-      vals[k] = 0;
-      if (s < n) {
-        const Item it = item_at(p, s, TPP);
-        vals[k] = ((it.len + 15) >> 4) * segs;
-        if (it.len == 0 && !it.skip) zero_item_output<HD>(p, it.row);
-      }
-      tsum += vals[k];
-    }
-    const int64_t inc = block_inclusive_scan<kPlanThreads>(tsum, wave_sums);
-    int64_t c = carry + inc - tsum;
-#pragma unroll
-    for (int k = 0; k < kPlanPer; ++k) {
-      const int64_t s = base + static_cast<int64_t>(tid) * kPlanPer + k;
-      if (s < n) p.cum[s] = c;
-      c += vals[k];
-    }
-    if (tid == kPlanThreads - 1) carry_sh = inc;
-    __syncthreads();
-    carry += carry_sh;
-    __syncthreads();
-  }
-  if (tid == 0) {
-    p.cum[n] = carry;
-    p.hdr[0] = carry;
-  }
-}
 
 // Item table of the in-LDS plan: length and page-table row of every item,
 // so a wavefront finds its next piece without a global round trip.

@@ -4,8 +4,10 @@
 // 2j and 2j + 1 of a page are two neighbouring blocks, [HD/x][TPP][x] keys and
 // [HD][TPP] values, so the pair's value is one [2 HD][TPP] block.
 //
-// One wavefront per (row, output head): lane t scores key k0 + t of both maps,
-// and then adds the block's values into the dims it owns, both maps' sums apart.
+// Decode rows (every row of the decode entry, the rows alone in their run of a
+// mixed batch) are streamed by diff_decode.h.  Rows of chunks: one wavefront per
+// (row, output head): lane t scores key k0 + t of both maps, and then adds the
+// block's values into the dims it owns, both maps' sums apart.
 #include "pal_device.h"
 
 namespace pal {
@@ -15,7 +17,7 @@ PAL_DEBUG_FLAGS_DEFINE(diff_debug_flags)
 
 }  // namespace pal
 
-#include "decode_plan.h"
+#include "diff_decode.h"
 
 namespace pal {
 
@@ -52,6 +54,7 @@ __global__ __launch_bounds__(kWave) void diff_rows_kernel(const DiffParams p, in
   int64_t seq = row, len = 0;
   if (p.q2seq) {
     const uint32_t sq = p.q2seq[row];
+    if ((row == 0 || p.q2seq[row - 1] != sq) && (row + 1 == p.num_seqs || p.q2seq[row + 1] != sq)) return;  // a lone row
     seq = sq < p.num_pt_rows ? sq : 0;
     if (sq < p.num_pt_rows) len = min(p.seq_lens[sq], p.q_offset[row]);
   } else {
@@ -136,33 +139,63 @@ __global__ __launch_bounds__(kWave) void diff_rows_kernel(const DiffParams p, in
   }
 }
 
-template <int DT, int HD, bool KV8>
-hipError_t launch_rows(const DiffParams& p, int tpp, hipStream_t stream) {
+template <int DT, int HD, int TPP, bool KV8>
+hipError_t launch_diff_t(const DiffParams& p, hipStream_t stream) {
+  if (p.num_seqs > kInlinePlanSeqs) {
+    hipLaunchKernelGGL((decode_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  hipLaunchKernelGGL((diff_stream_kernel<DT, HD, TPP, KV8>), dim3(static_cast<unsigned>(p.num_workers / kDiffWaves)),
+                     dim3(kDiffThreads), 0, stream, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL((diff_merge_kernel<DT, HD>), dim3(static_cast<unsigned>(p.num_workers), static_cast<unsigned>(p.hg_max)),
+                     dim3(kDiffThreads), 0, stream, p);
+  err = hipGetLastError();
+  if (err != hipSuccess || !p.q2seq) return err;
   const int64_t groups = p.num_seqs * (p.num_q_heads / 2);
   if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((diff_rows_kernel<DT, HD, KV8>), dim3(static_cast<unsigned>(groups)), dim3(kWave), 0, stream, p, tpp);
+  hipLaunchKernelGGL((diff_rows_kernel<DT, HD, KV8>), dim3(static_cast<unsigned>(groups)), dim3(kWave), 0, stream, p, TPP);
   return hipGetLastError();
+}
+
+template <int DT, int HD, bool KV8>
+hipError_t launch_tpp(const DiffParams& p, int tpp, hipStream_t stream) {
+  switch (tpp) {
+    case 16: return launch_diff_t<DT, HD, 16, KV8>(p, stream);
+    case 32: return launch_diff_t<DT, HD, 32, KV8>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 template <int DT>
 hipError_t launch_hd(const DiffParams& p, int hd, int tpp, hipStream_t stream) {
   if (p.k_scales) {
     switch (hd) {
-      case 64: return launch_rows<DT, 64, true>(p, tpp, stream);
-      case 128: return launch_rows<DT, 128, true>(p, tpp, stream);
+      case 64: return launch_tpp<DT, 64, true>(p, tpp, stream);
+      case 128: return launch_tpp<DT, 128, true>(p, tpp, stream);
       default: return hipErrorInvalidValue;
     }
   }
   switch (hd) {
-    case 32: return launch_rows<DT, 32, false>(p, tpp, stream);
-    case 64: return launch_rows<DT, 64, false>(p, tpp, stream);
-    case 96: return launch_rows<DT, 96, false>(p, tpp, stream);
-    case 128: return launch_rows<DT, 128, false>(p, tpp, stream);
+    case 32: return launch_tpp<DT, 32, false>(p, tpp, stream);
+    case 64: return launch_tpp<DT, 64, false>(p, tpp, stream);
+    case 96: return launch_tpp<DT, 96, false>(p, tpp, stream);
+    case 128: return launch_tpp<DT, 128, false>(p, tpp, stream);
     default: return hipErrorInvalidValue;
   }
 }
 
 }  // namespace
+
+hipError_t diff_resident_workers(int* workers) {
+  int dev = 0, cus = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err == hipSuccess) err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  *workers = cus * kDiffWaves;  // one workgroup per CU
+  return err;
+}
 
 hipError_t launch_diff(const DiffParams& p, int dtype, int head_dim, int tokens_per_page, hipStream_t stream) {
   if (dtype == kBF16) return launch_hd<kBF16>(p, head_dim, tokens_per_page, stream);

@@ -1,0 +1,643 @@
+// Differential attention of single rows (decode rows) over the paged cache: the
+// device code of the stream over the cache and of the merge behind it.
+//
+// For output head i with maps 1, 2 (query heads 2i, 2i + 1) and kv pair j (kv
+// heads 2j, 2j + 1: two neighbouring (page, kv head) blocks of either pool):
+//   O_m = sum_t e^(s_m,t - M_m) V_t,  l_m = sum_t e^(s_m,t - M_m),  s_m = q_m K_m^T / sqrt(HD)
+//   x = O_1 / l_1 - lambda O_2 / l_2,  y = out_scale w x / sqrt(mean(x^2) + eps)
+// in one pass over the keys with running maxima, the two maps' states apart
+// (their exp-sums' ratio is known only at the end).
+//
+// Mapping: ordinary decode's (decode.hip), with the pair for the kv head.  The
+// list of all 16-token blocks of the batch is cut into equal shares, one per
+// resident wavefront; a wavefront streams its blocks with the loads of the next
+// ones in flight, and split segments leave partials.  What differs:
+//  * Up to 8 output heads of a kv pair are the 16 columns of the products:
+//    columns 0..7 their first maps, 8..15 their second.  Both keys are multiplied
+//    with all columns and each lane keeps the product that is its map's: as many
+//    MFMAs as ordinary decode has for two kv heads, and an infinite key of one
+//    map cannot reach the other (as zero-padded queries of 2 HD dims would let
+//    it).  The value's 2 HD rows are then read once for both maps.
+//  * The maps of a head sit in lanes r and r ^ 8, so the difference of a finished
+//    segment is one lane rotation per value, and the norm's sum stays in the
+//    wavefront.
+//  * Partials hold O, its maximum and exp-sum in fp32: the difference of two maps
+//    may be small against either, and a partial rounded to 16 bits, as ordinary
+//    decode keeps it, would cost 2^-8 of the maps.
+#pragma once
+
+#include "decode_plan.h"
+
+namespace pal {
+namespace {
+
+constexpr int kDiffWaves = 4;  // independent wavefront workers per workgroup
+constexpr int kDiffThreads = kDiffWaves * kWave;
+constexpr float kDiffLazyMax = 8.f;  // log2 headroom before a running max moves
+
+// The items of a batch of up to kInlinePlanSeqs, in LDS.
+struct DiffPlanLds {
+  int64_t cum[kInlinePlanSeqs + 1];
+  int32_t len[kInlinePlanSeqs];
+  int32_t seq[kInlinePlanSeqs];
+  int64_t wave_sums[kDiffWaves];
+};
+
+// x's value in lane l ^ 8 (a rotation by 8 of each 16 lanes)
+__device__ __forceinline__ float lane_xor8(float x) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x128, 0xf, 0xf, true));  // row_ror:8
+}
+
+// Streams the blocks of virtual worker v.  The blocks form a run of pieces (the
+// blocks of one segment inside the worker's range); the pipeline runs through
+// piece boundaries: while the last blocks of a piece are computed, the first
+// of the next piece are loading (its item, query and first page ids were fetched
+// when the piece before it started).
+template <int DT, int HD, int TPP, int PF, bool KV8>
+__device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc, const int64_t* cum,
+                                           const DiffPlanLds* plan, int64_t v) {
+  static_assert(HD % 32 == 0 && (!KV8 || HD % 64 == 0), "whole k-steps and stripes");
+  constexpr int KK = HD / 32;     // QK k-steps of 32 dims of one map
+  constexpr int NT = 2 * HD / 16;  // output tiles of 16 dims
+  constexpr int NBUF = PF + 1;
+  constexpr int EB = KV8 ? 1 : 2;  // pool element bytes
+  constexpr int KL = KV8 ? HD / 64 : KK;  // 16-byte key loads of one map
+
+  const int64_t b0 = vstart(sc, v);
+  const int64_t b_end = vstart(sc, v + 1);
+  const int lane = lane_id();
+  // the split segment whose first piece ends the worker's range, or none
+  int64_t list_g0 = -1, list_nb = 0, list_row = 0, list_seg = 0;
+  auto write_list = [&] {
+    if (lane == 0) {
+      int64_t* slot = p.split_list + 4 * v;
+      slot[0] = list_g0;
+      slot[1] = list_nb;
+      slot[2] = list_row;
+      slot[3] = list_seg;
+    }
+  };
+  if (b_end <= b0) {
+    write_list();
+    return;
+  }
+
+  const int g = lane >> 4;
+  const int r16 = lane & 15;
+  const int map = r16 >> 3;  // this lane's column: map, and head of the chunk
+  const int r8 = r16 & 7;
+  const int segs = p.num_kv_heads * p.head_chunks;
+  const int64_t head_block = static_cast<int64_t>(HD) * TPP * EB;  // bytes per (page, kv head)
+  const int64_t page_stride = head_block * 2 * p.num_kv_heads;
+
+  // A piece: item s (of page-table row `seq`, `len` keys, nb blocks per segment),
+  // segment `seg`, blocks [blk, blk + count) of the segment, from global block
+  // gpos on; r = block offset of the piece inside the item's segments.  c_* is
+  // the piece being computed, x_* the next one (kept in scalars).
+  int64_t c_s, c_r, c_gpos, c_seq, c_len, c_nb, c_blk, c_count;
+  int c_seg;
+  int64_t x_s, x_r, x_gpos, x_seq, x_len, x_nb, x_blk, x_count;
+  int x_seg;
+#define PAL_FIND_PIECE(P, S0, R0, G0)                                                      \
+  do {                                                                                     \
+    int64_t s_ = (S0), r_ = (R0), len_, seq_;                                              \
+    for (;;) {                                                                             \
+      if (plan) {                                                                          \
+        len_ = plan->len[s_];                                                              \
+        seq_ = plan->seq[s_];                                                              \
+      } else {                                                                             \
+        const Item it_ = item_at(p, s_, TPP);                                              \
+        len_ = it_.len;                                                                    \
+        seq_ = it_.seq;                                                                    \
+      }                                                                                    \
+      if (len_ > 0) break;                                                                 \
+      ++s_;                                                                                \
+      r_ = 0;                                                                              \
+    }                                                                                      \
+    P##s = s_;                                                                             \
+    P##r = r_;                                                                             \
+    P##gpos = (G0);                                                                        \
+    P##seq = seq_;                                                                         \
+    P##len = len_;                                                                         \
+    P##nb = (len_ + 15) >> 4;                                                              \
+    P##seg = static_cast<int>(r_ / P##nb);                                                 \
+    P##blk = r_ - P##seg * P##nb;                                                          \
+    P##count = (P##nb - P##blk) < (b_end - P##gpos) ? (P##nb - P##blk) : (b_end - P##gpos); \
+  } while (0)
+
+  // Q^T operand of a piece: the dims of this lane's k-slices of its column's
+  // query (zeros in columns without a head).
+  u32x4 qv[KK], qn[KK];
+  auto load_q = [&](int64_t s, int seg, u32x4 (&q)[KK]) {
+    const int h0 = (seg % p.head_chunks) * 8;
+    const bool hv = r8 < min(8, p.group - h0);
+    const uint32_t qmask = hv ? 0xFFFFFFFFu : 0u;
+    const int64_t head = static_cast<int64_t>(seg / p.head_chunks) * p.group + h0 + (hv ? r8 : 0);
+    const uint16_t* qrow = p.q + (s * p.num_q_heads + 2 * head + map) * HD;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (KV8)  // k-step kk = (stripe g + 4 (kk / 2), half kk % 2)
+        q[kk] = *reinterpret_cast<const u32x4*>(qrow + 16 * (g + 4 * (kk >> 1)) + 8 * (kk & 1)) & qmask;
+      else
+        q[kk] = *reinterpret_cast<const u32x4*>(qrow + 32 * kk + 8 * g) & qmask;
+    }
+  };
+  // page ids of window wi (64 pages, one per lane) of a piece
+  auto load_window = [&](int64_t seq, int64_t blk, int64_t wi) {
+    const uint32_t* pt = p.page_table + seq * p.page_table_width;
+    int64_t lp = (blk * 16) / TPP + wi * kWave + lane;
+    if (lp >= p.page_table_width) lp = p.page_table_width - 1;
+    return pt[lp];
+  };
+  {
+    const int64_t s0 = locate_seq(cum, p.num_seqs, b0);  // the item holding block b0 (it has blocks)
+    PAL_FIND_PIECE(c_, s0, b0 - cum[s0], b0);
+  }
+  load_q(c_s, c_seg, qv);
+
+  // Page ids in register windows of 64 pages: pid_cur holds window wcur, the
+  // window of the block being computed, pid_nxt the next one; every step group
+  // also loads the one after that, and the windows move up when the computed
+  // block enters window wcur + 1.
+  int wcur = 0;
+  uint32_t pid_cur = load_window(c_seq, c_blk, 0), pid_nxt = load_window(c_seq, c_blk, 1),
+           pid_later = load_window(c_seq, c_blk, 2);
+
+  u32x4 kb[NBUF][2][KL];
+  u32x2 vb[NBUF][KV8 ? 1 : NT];
+  u32x4 vq8[NBUF][KV8 ? NT / 4 : 1];
+  f32x2 bks[NBUF], bvs[NBUF];  // fp8: the block's scales, of kv heads 2j and 2j + 1
+  bool bv[NBUF];
+
+  bool first = true;     // the piece is the worker's first
+  bool prologue = true;  // the pipeline is empty
+  bool has_next = false;
+  x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
+  x_count = c_count; x_seg = c_seg;
+  uint32_t pidn0 = 0;        // window 0 of the next piece (a load in flight)
+  uint32_t pidn0_ready = 0;  // the same once it has arrived (see below)
+
+  for (;;) {
+    const int pair = c_seg / p.head_chunks;
+    const int h0 = (c_seg % p.head_chunks) * 8;
+    const int hg = min(8, p.group - h0);
+    const bool complete = (c_blk == 0) && (c_count == c_nb);
+    const int len = static_cast<int>(c_len);
+    const int n_blk = static_cast<int>(c_count);
+    const int n_pad = (n_blk + NBUF - 1) / NBUF * NBUF;  // steps of the piece
+    const int bstart = static_cast<int>(c_blk);
+    const int pbase = (bstart * 16) / TPP;
+    const uint8_t* kbase = static_cast<const uint8_t*>(p.k_pool) + pair * 2 * head_block;
+    const uint8_t* vbase = static_cast<const uint8_t*>(p.v_pool) + pair * 2 * head_block;
+    const uint8_t* kbase_n = kbase;  // set once the next piece is known
+    const uint8_t* vbase_n = vbase;
+    int pair_n = pair;
+    int nblk_n = 1;
+    int bstart_n = 0, pbase_n = 0;
+
+    // Issues the loads of step i of the piece into buffer `buf`: block i of the
+    // piece (clamped to its last) or, past the piece's steps, block i - n_pad of
+    // the next piece.  An out-of-range page id reads page 0 and the block is
+    // masked when computed.  Every block is read once per call: non-temporal,
+    // but for 32-token pages, whose rows this block and the next share (as in
+    // ordinary decode: cacheable where a kv head's block holds 8 KiB or more).
+    constexpr bool kCached = TPP == 32 && 2 * HD * TPP * EB >= 8192;
+    auto load16 = [](const uint8_t* a) {
+      if constexpr (kCached) return *reinterpret_cast<const u32x4*>(a);
+      else return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a));
+    };
+    auto load8 = [](const uint8_t* a) {
+      if constexpr (kCached) return *reinterpret_cast<const u32x2*>(a);
+      else return __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(a));
+    };
+    auto issue = [&](int i, int buf, uint32_t w_n0) {
+      const bool to_next = has_next && i >= n_pad;
+      const int j = to_next ? (i - n_pad < nblk_n - 1 ? i - n_pad : nblk_n - 1) : (i < n_blk - 1 ? i : n_blk - 1);
+      const int b = (to_next ? bstart_n : bstart) + j;
+      const int e = (b * 16) / TPP - (to_next ? pbase_n : pbase);  // page within the piece's windows
+      // (selects of values: a select of two variables' addresses would push the
+      // pipeline state to scratch)
+      const uint32_t w_c = pid_cur, w_x = pid_nxt;
+      const uint32_t win = to_next ? w_n0 : ((e >> 6) == wcur ? w_c : w_x);
+      const uint32_t pg = __builtin_amdgcn_readlane(win, static_cast<int>(e & 63));
+      bv[buf] = pg < p.num_pages;
+      PAL_DEBUG_FLAG(!bv[buf] && (to_next ? i - n_pad < nblk_n : i < n_blk), kDebugPageId);
+      const uint32_t page = bv[buf] ? pg : 0u;
+      const int slot0 = static_cast<int>((b * 16) % TPP);
+      const uint8_t* kb_x = kbase_n;
+      const uint8_t* vb_x = vbase_n;
+      const uint8_t* kp = (to_next ? kb_x : kbase) + static_cast<int64_t>(page) * page_stride + (slot0 + r16) * 16;
+      const uint8_t* vp = (to_next ? vb_x : vbase) + static_cast<int64_t>(page) * page_stride + slot0 * EB;
+      if constexpr (KV8) {
+        const int64_t si = 2 * (static_cast<int64_t>(page) * p.num_kv_heads + (to_next ? pair_n : pair));
+        bks[buf] = f32x2{p.k_scales[si], p.k_scales[si + 1]};
+        bvs[buf] = f32x2{p.v_scales[si], p.v_scales[si + 1]};
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int kk = 0; kk < KL; ++kk) kb[buf][a][kk] = load16(kp + a * head_block + (4 * kk + g) * TPP * 16);
+      if constexpr (KV8) {
+        // lane 16g + i reads the block's 16 codes of dim row 64q + 16g + i; compute
+        // transposes them across the lane groups
+#pragma unroll
+        for (int q = 0; q < NT / 4; ++q) vq8[buf][q] = load16(vp + (64 * q + 16 * g + r16) * TPP);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) vb[buf][n] = load8(vp + ((16 * n + r16) * TPP + 4 * g) * 2);
+      }
+    };
+
+    float m_run = -INFINITY;  // running max of this lane's column (log2 units)
+    float l_run = 0.f;        // this lane's share of its exp-sum
+    f32x4 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto compute = [&](int i, int buf) {
+      const int b = bstart + i;
+      const bool live = bv[buf] && i < n_blk;  // steps past the piece end are fully masked
+      f32x4 acc[2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          if constexpr (KV8) {
+            const u32x4 w = kb[buf][a][kk / 2];
+            acc[a] = Dt<DT>::mma16x16x32(fp8x8_exact<DT>(kk % 2 ? u32x2{w.z, w.w} : u32x2{w.x, w.y}), qv[kk], acc[a]);
+          } else {
+            acc[a] = Dt<DT>::mma16x16x32(kb[buf][a][kk], qv[kk], acc[a]);
+          }
+        }
+      }
+      const float ks = KV8 ? (map ? bks[buf].y : bks[buf].x) * p.scale_log2 : p.scale_log2;
+      // tokens past the end (and whole invalid blocks) are masked: token 4g + e of
+      // the block is a key when e < kl
+      const int left = live ? len - b * 16 : 0;
+      const int kl = static_cast<int>(left < 16 ? left : 16) - 4 * g;
+      float sc4[4];
+      float bm = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float s = (map ? acc[1][e] : acc[0][e]) * ks;
+        sc4[e] = e < kl ? s : -INFINITY;
+        bm = fmaxf(bm, sc4[e]);
+      }
+      // the running max of a column moves only when a score passes it by more
+      // than the headroom (always for its first score above -inf)
+      if (__ballot(bm > m_run + kDiffLazyMax)) {
+        const float m_new = fmaxf(m_run, max_xor32(max_xor16(bm)));
+        const float alpha = (m_new == -INFINITY) ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n] *= alpha;
+        m_run = m_new;
+      }
+      const float mref = (m_run == -INFINITY) ? 0.f : m_run;
+      float pe[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pe[e] = __builtin_amdgcn_exp2f(sc4[e] - mref);
+        l_run += pe[e];
+      }
+      // The probabilities are rounded to the pool's 16-bit type for the product
+      // (fp8: with the value scale of the half's kv head on them; the exp-sum
+      // takes them unrounded and unscaled).
+      u32x2 pb[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float f = KV8 ? bvs[buf][hf] : 1.f;
+        pb[hf] = u32x2{Dt<DT>::pack2(pe[0] * f, pe[1] * f), Dt<DT>::pack2(pe[2] * f, pe[3] * f)};
+      }
+      // slots past the end may hold anything, NaN bits included: zero their values
+      const uint32_t mlo = (kl > 0 ? 0x0000FFFFu : 0u) | (kl > 1 ? 0xFFFF0000u : 0u);
+      const uint32_t mhi = (kl > 2 ? 0x0000FFFFu : 0u) | (kl > 3 ? 0xFFFF0000u : 0u);
+      const uint32_t m8 = kl >= 4 ? 0xFFFFFFFFu : (kl <= 0 ? 0u : (0xFFFFFFFFu >> (32 - 8 * kl)));
+      u32x4 vt[KV8 ? NT / 4 : 1];
+      if constexpr (KV8) {
+#pragma unroll
+        for (int q = 0; q < NT / 4; ++q) vt[q] = transpose_lane_groups4(vq8[buf][q]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        u32x2 vv;
+        if constexpr (KV8) {
+          const uint32_t codes = vt[n >> 2][n & 3] & m8;  // a zero code is +0
+          vv = u32x2{Dt<DT>::fp8x2(codes, false), Dt<DT>::fp8x2(codes, true)};
+        } else {
+          vv = u32x2{vb[buf][n].x & mlo, vb[buf][n].y & mhi};
+        }
+        o[n] = Dt<DT>::mma16x16x16(vv, pb[KV8 ? n / (NT / 2) : 0], o[n]);
+      }
+    };
+
+    // The first piece fills the pipeline; a later one finds its first PF blocks
+    // in flight.
+    if (prologue) {
+#pragma unroll
+      for (int q = 0; q < PF; ++q) issue(q, q, pidn0);  // (never the next piece)
+    }
+
+    // The next piece: its item, query and first page ids load now, while this
+    // piece streams (with none, the current one's again: no load under a branch).
+    {
+      const int64_t gpos_n = c_gpos + c_count;
+      has_next = gpos_n < b_end;
+      int64_t s_n = c_s, r_n = c_r + c_count;
+      if (r_n >= c_nb * segs) {
+        ++s_n;
+        r_n = 0;
+      }
+      if (has_next) {
+        PAL_FIND_PIECE(x_, s_n, r_n, gpos_n);
+      } else {
+        x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
+        x_count = c_count; x_seg = c_seg;
+      }
+      load_q(x_s, x_seg, qn);
+      pidn0 = load_window(x_seq, x_blk, 0);
+    }
+    const uint32_t pidn1 = load_window(x_seq, x_blk, 1);
+    {
+      pair_n = x_seg / p.head_chunks;
+      kbase_n = static_cast<const uint8_t*>(p.k_pool) + pair_n * 2 * head_block;
+      vbase_n = static_cast<const uint8_t*>(p.v_pool) + pair_n * 2 * head_block;
+      nblk_n = static_cast<int>(x_count);
+      bstart_n = static_cast<int>(x_blk);
+      pbase_n = (bstart_n * 16) / TPP;
+    }
+
+    // Every step issues and computes unconditionally (steps past the end re-read
+    // the last block and compute it fully masked), so the compiler's wait counts
+    // stay exact and the blocks in flight are never drained early.  The groups of
+    // a piece with two or more of them select the next piece's window from
+    // pidn0_ready, refreshed at the end of each group where the wait is exact:
+    // selecting pidn0 would wait for that load at the top of every group.
+    auto step_group = [&](int i0, uint32_t w_n0) {
+      const uint32_t pid_ahead = load_window(c_seq, c_blk, wcur + 2);
+#pragma unroll
+      for (int u = 0; u < NBUF; ++u) {
+        const int i = i0 + u;
+        issue(i + PF, (u + PF) % NBUF, w_n0);
+        compute(i, u);
+      }
+      const int e_last = ((bstart + i0 + NBUF - 1) * 16) / TPP - pbase;
+      const bool up = (e_last >> 6) > wcur;
+      pid_cur = up ? pid_nxt : pid_cur;
+      pid_nxt = up ? pid_later : pid_nxt;
+      wcur += up ? 1 : 0;
+      pid_later = pid_ahead;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(qn[kk]));
+      asm volatile("" ::"v"(pidn1));
+      asm volatile("v_mov_b32 %0, %1" : "=v"(pidn0_ready) : "v"(pidn0));
+    };
+    if (n_pad == NBUF) {
+      step_group(0, pidn0);
+    } else {
+      int i0 = 0;
+      do {
+        step_group(i0, pidn0_ready);
+        i0 += NBUF;
+      } while (i0 < n_pad);
+    }
+
+    // ---- finish the piece: exp-sum of the column over the 4 lane groups
+    const float l = sum_xor32(sum_xor16(l_run));
+    if (complete) {
+      // x = O_1 / l_1 - lambda O_2 / l_2: each lane adds its map's term to that of
+      // lane ^ 8, so both hold x; the norm sums it over the 4 lane groups
+      const int64_t head = static_cast<int64_t>(pair) * p.group + h0 + (r8 < hg ? r8 : 0);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // (no score above -inf: the map adds nothing)
+      const float f = map ? -p.lambdas[head] * inv : inv;
+      float ss = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float t = o[n][e] * f;
+          o[n][e] = t + lane_xor8(t);
+          ss += o[n][e] * o[n][e];
+        }
+      }
+      float scale = p.out_scale;
+      if (p.norm_weight) scale *= 1.f / sqrtf(sum_xor32(sum_xor16(ss)) * (1.f / (2 * HD)) + p.norm_eps);
+      if (r8 < hg) {
+        // the two lanes of a head write half of its row each
+        uint16_t* row = p.out + (c_s * (p.num_q_heads / 2) + head) * (2 * HD) + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+          const int t = n + map * (NT / 2);
+          f32x4 y = map ? o[n + NT / 2] : o[n];
+          y *= scale;
+          if (p.norm_weight) y *= *reinterpret_cast<const f32x4*>(p.norm_weight + 16 * t + 4 * g);
+          *reinterpret_cast<u32x2*>(row + 16 * t) = u32x2{Dt<DT>::pack2(y[0], y[1]), Dt<DT>::pack2(y[2], y[3])};
+        }
+      }
+    } else {
+      if (r8 < hg) {
+        const int64_t slot = ((v * 2 + (first ? 0 : 1)) * 2 + map) * p.hg_max + r8;
+        float* po = p.part_o32 + slot * (2 * HD) + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(po + 16 * n) = o[n];
+        if (g == 0) *reinterpret_cast<f32x2*>(p.part_ml + slot * 2) = f32x2{m_run, l};
+      }
+      if (c_blk == 0) {  // the first piece of a split segment ends the worker's range
+        list_g0 = c_gpos;
+        list_nb = c_nb;
+        list_row = c_s;
+        list_seg = c_seg;
+      }
+    }
+    prologue = false;
+    first = false;
+    if (!has_next) break;
+    // the next piece becomes current: its first PF blocks are in flight, in
+    // buffers 0 .. PF-1 (n_pad is a multiple of NBUF)
+    c_s = x_s; c_r = x_r; c_gpos = x_gpos; c_seq = x_seq; c_len = x_len; c_nb = x_nb; c_blk = x_blk;
+    c_count = x_count; c_seg = x_seg;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qv[kk] = qn[kk];
+    wcur = 0;
+    pid_cur = pidn0;
+    pid_nxt = pidn1;
+    pid_later = load_window(c_seq, c_blk, 2);
+  }
+  write_list();
+#undef PAL_FIND_PIECE
+}
+
+template <int DT, int HD, int TPP, bool KV8>
+__global__ __launch_bounds__(kDiffThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void diff_stream_kernel(const DiffParams p) {
+  __shared__ DiffPlanLds lds;
+  const int64_t n = p.num_seqs;
+  const bool lds_plan = n <= kInlinePlanSeqs;
+  const int64_t* cum = p.cum;
+  int64_t total;
+  if (lds_plan) {
+    // every workgroup scans the lengths into LDS: thread t owns items 4t .. 4t+3
+    constexpr int kPer = kInlinePlanSeqs / kDiffThreads;
+    const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
+    const int tid = threadIdx.x;
+    int64_t vals[kPer];
+    int64_t tsum = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t s = static_cast<int64_t>(tid) * kPer + k;
+      vals[k] = 0;
+      if (s < n) {
+        const Item it = item_at(p, s, TPP);
+        vals[k] = ((it.len + 15) >> 4) * segs;
+        lds.len[s] = static_cast<int32_t>(it.len);
+        lds.seq[s] = static_cast<int32_t>(it.seq);
+        if (it.len == 0 && !it.skip && blockIdx.x == 0) zero_item_output<HD>(p, it.row);
+      }
+      tsum += vals[k];
+    }
+    const int64_t incl = block_inclusive_scan<kDiffThreads>(tsum, lds.wave_sums);
+    int64_t c = incl - tsum;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t s = static_cast<int64_t>(tid) * kPer + k;
+      if (s < n) lds.cum[s] = c;
+      c += vals[k];
+    }
+    if (tid == kDiffThreads - 1) lds.cum[n] = incl;
+    __syncthreads();
+    total = lds.cum[n];
+    if (blockIdx.x == 0 && tid == 0) p.hdr[0] = total;
+    cum = lds.cum;
+  } else {
+    total = p.hdr[0];
+  }
+  if (total == 0) return;
+  const Sched sc = make_sched(total, p.num_workers, 0);
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kDiffWaves + wave_id();
+  if (w < sc.nws) diff_range<DT, HD, TPP, KV8 ? 3 : 2, KV8>(p, sc, cum, lds_plan ? &lds : nullptr, w);
+}
+
+// Joins the pieces of split segments: workgroup (v, h) takes head h of the
+// segment in list slot v, whose first piece is worker v's, further pieces the
+// first ones of workers v + 1, v + 2, ...  A wavefront takes every fourth piece
+// (times the rows one 16-byte load per lane covers), all maxima first:
+//   O_m = sum_c 2^(M_c - M) O_c,  l_m = sum_c 2^(M_c - M) l_c
+// the wavefronts' sums meet in LDS, and the first finishes the row.
+template <int DT, int HD>
+__global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffParams p) {
+  constexpr int D = 2 * HD;
+  constexpr int kLpr = D <= 64 ? 16 : (D <= 128 ? 32 : 64);  // lanes per partial row, 4 dims each
+  constexpr int kRows = kWave / kLpr;                        // rows of one load
+  constexpr int kBatch = 4;
+  __shared__ __attribute__((aligned(16))) float sum_lds[kDiffWaves][2][D];
+  __shared__ float l_lds[kDiffWaves][2];
+  const int64_t e = blockIdx.x;
+  const int h = blockIdx.y;
+  const int64_t total = p.hdr[0];
+  const int64_t* slot = p.split_list + 4 * e;
+  const int64_t g0 = slot[0], nb = slot[1], row = slot[2];
+  const int seg = static_cast<int>(slot[3]);
+  if (total == 0) return;
+  const Sched sc = make_sched(total, p.num_workers, 0);
+  if (e >= sc.nws || g0 < 0) return;
+  const int h0 = (seg % p.head_chunks) * 8;
+  if (h >= min(8, p.group - h0)) return;
+  const int head = (seg / p.head_chunks) * p.group + h0 + h;
+  const int nc = static_cast<int>(vworker_of(sc, g0 + nb - 1) - e) + 1;
+  const int t0 = vstart(sc, e) >= g0 ? 0 : 1;  // the first piece's partial slot
+  const int lane = lane_id();
+  const int w = wave_id();
+  const int rl = lane % kLpr;
+  const int rg = lane / kLpr;
+  const bool dl = 4 * rl < D;
+  auto row_of = [&](int c, int map) { return (((e + c) * 2 + (c == 0 ? t0 : 0)) * 2 + map) * p.hg_max + h; };
+
+  float big[2] = {-INFINITY, -INFINITY};
+  for (int c = lane; c < nc; c += kWave) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) big[m] = fmaxf(big[m], p.part_ml[row_of(c, m) * 2]);
+  }
+  float ref[2], l[2] = {0.f, 0.f};
+  f32x4 acc[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) big[m] = fmaxf(big[m], shfl_xor(big[m], off));
+    ref[m] = big[m] == -INFINITY ? 0.f : big[m];
+    acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int c0 = w * kRows; c0 < nc; c0 += kDiffWaves * kRows * kBatch) {
+    f32x2 ml[kBatch][2];
+    f32x4 o[kBatch][2];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * kDiffWaves * kRows + rg;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int64_t r = row_of(c < nc ? c : nc - 1, m);  // (past the last: read again, weight 0)
+        ml[u][m] = *reinterpret_cast<const f32x2*>(p.part_ml + r * 2);
+        o[u][m] = *reinterpret_cast<const f32x4*>(p.part_o32 + r * D + (dl ? 4 * rl : 0));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (c0 + u * kDiffWaves * kRows + rg < nc) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const float f = __builtin_amdgcn_exp2f(ml[u][m].x - ref[m]);
+          l[m] += f * ml[u][m].y;
+          acc[m] += f * o[u][m];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int off = kLpr; off < kWave; off <<= 1) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      l[m] += shfl_xor(l[m], off);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][i] += shfl_xor(acc[m][i], off);
+    }
+  }
+  if (rg == 0 && dl) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) *reinterpret_cast<f32x4*>(&sum_lds[w][m][4 * rl]) = acc[m];
+  }
+  if (lane == 0) {
+    l_lds[w][0] = l[0];
+    l_lds[w][1] = l[1];
+  }
+  __syncthreads();
+  if (w != 0) return;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    float lm = 0.f;
+    f32x4 om = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < kDiffWaves; ++u) {
+      lm += l_lds[u][m];
+      om += *reinterpret_cast<const f32x4*>(&sum_lds[u][m][dl ? 4 * rl : 0]);
+    }
+    const float inv = lm > 0.f || lm != lm ? 1.f / lm : 0.f;
+    x += om * (m ? -p.lambdas[head] * inv : inv);
+  }
+  float scale = p.out_scale;
+  if (p.norm_weight) {
+    float ss = rg == 0 && dl ? x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3] : 0.f;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) ss += shfl_xor(ss, off);
+    scale *= 1.f / sqrtf(ss * (1.f / D) + p.norm_eps);
+  }
+  if (rg == 0 && dl) {
+    f32x4 y = x * scale;
+    if (p.norm_weight) y *= *reinterpret_cast<const f32x4*>(p.norm_weight + 4 * rl);
+    *reinterpret_cast<u32x2*>(p.out + (row * (p.num_q_heads / 2) + head) * D + 4 * rl) =
+        u32x2{Dt<DT>::pack2(y[0], y[1]), Dt<DT>::pack2(y[2], y[3])};
+  }
+}
+
+}  // namespace
+}  // namespace pal

@@ -615,13 +615,37 @@ int check_diff_dims(const char* op, int dtype, int kv_dtype, int num_q_heads, in
   return PAL_OK;
 }
 
+// Workspace layout of a differential attention call (256-byte aligned offsets);
+// nothing in it needs initial contents.
+struct DiffLayout {
+  size_t cum, list, part_ml, part_o, total;
+};
+
+DiffLayout diff_layout(int64_t num_rows, int head_dim, int hg_max, int workers) {
+  const size_t rows = static_cast<size_t>(workers) * 2 * 2 * hg_max;  // partial rows
+  DiffLayout l;
+  l.cum = 256;  // behind the header
+  l.list = l.cum + align256(static_cast<size_t>(num_rows + 1) * sizeof(int64_t));
+  l.part_ml = l.list + align256(static_cast<size_t>(workers) * 4 * sizeof(int64_t));
+  l.part_o = l.part_ml + align256(rows * 2 * sizeof(float));
+  l.total = l.part_o + align256(rows * 2 * head_dim * sizeof(float));
+  return l;
+}
+
+int diff_heads_per_segment(int num_q_heads, int num_kv_heads) {
+  const int group = num_q_heads / num_kv_heads;
+  return group < 8 ? group : 8;
+}
+
 size_t diff_workspace_size(int dtype, int kv_dtype, int64_t num_rows, int num_q_heads, int num_kv_heads, int head_dim,
                            int tokens_per_page) {
+  int workers = 0;
   if (num_rows <= 0 || num_rows > 0x7fffffffLL ||
       check_diff_dims("paged_differential_attention", dtype, kv_dtype, num_q_heads, num_kv_heads, head_dim,
-                      tokens_per_page, 0, 0) != PAL_OK)
+                      tokens_per_page, 0, 0) != PAL_OK ||
+      pal::diff_resident_workers(&workers) != hipSuccess)
     return 0;
-  return 256;
+  return diff_layout(num_rows, head_dim, diff_heads_per_segment(num_q_heads, num_kv_heads), workers).total;
 }
 
 // Rows of sequences: row i of sequence i (decode: no map), or of query_to_seq_map[i].
@@ -649,9 +673,14 @@ int diff_call(const char* op, bool mapped, const void* queries, const void* k_po
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] null pointer argument", op);
   if (!aligned16(queries) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(norm_weight) || !aligned16(out))
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] queries, pools, norm_weight and out must be 16-byte aligned", op);
-  const size_t need = diff_workspace_size(dtype, kv_dtype, num_rows, num_q_heads, num_kv_heads, head_dim, tokens_per_page);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace of %zu bytes needed, %zu given", op, need, workspace_bytes);
+  int workers = 0;
+  const hipError_t err = pal::diff_resident_workers(&workers);
+  if (err != hipSuccess) return hip_status(err, op);
+  const int hg_max = diff_heads_per_segment(num_q_heads, num_kv_heads);
+  const DiffLayout lay = diff_layout(num_rows, head_dim, hg_max, workers);
+  if (workspace == nullptr || workspace_bytes < lay.total)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace of %zu bytes needed, %zu given", op, lay.total,
+                workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u)
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace must be 256-byte aligned", op);
   pal::DiffParams p{};
@@ -673,8 +702,16 @@ int diff_call(const char* op, bool mapped, const void* queries, const void* k_po
   p.num_kv_heads = num_kv_heads / 2;
   p.group = num_q_heads / num_kv_heads;
   p.head_chunks = (p.group + 7) / 8;
-  p.hg_max = p.group < 8 ? p.group : 8;
+  p.hg_max = hg_max;
+  p.num_workers = workers;
   p.scale_log2 = scale_log2_for(head_dim);
+  char* ws = static_cast<char*>(workspace);
+  p.hdr = reinterpret_cast<int64_t*>(ws);
+  p.cum = reinterpret_cast<int64_t*>(ws + lay.cum);
+  p.split_list = reinterpret_cast<int64_t*>(ws + lay.list);
+  p.list_cap = workers;
+  p.part_ml = reinterpret_cast<float*>(ws + lay.part_ml);
+  p.part_o32 = reinterpret_cast<float*>(ws + lay.part_o);
   p.lambdas = lambdas;
   p.norm_weight = norm_weight;
   p.norm_eps = norm_eps;

@@ -182,7 +182,11 @@ struct DiffParams : DecodeParams {
   const float* norm_weight;  // [2 HD], or null: no norm
   float norm_eps;
   float out_scale;
+  float* part_o32;           // [virtual workers][2][2 maps][hg_max][2 HD], not normalised (part_ml likewise: max, exp-sum)
 };
+
+// Wavefront workers that stream decode rows (one workgroup per CU of the current device).
+hipError_t diff_resident_workers(int* workers);
 
 hipError_t launch_diff(const DiffParams& p, int dtype, int head_dim, int tokens_per_page, hipStream_t stream);
 
