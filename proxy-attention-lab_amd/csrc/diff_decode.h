@@ -21,6 +21,8 @@
 //  * The maps of a head sit in lanes r and r ^ 8, so the difference of a finished
 //    segment is one lane rotation per value, and the norm's sum stays in the
 //    wavefront.
+//  * The probabilities enter the product with the values as two 16-bit terms, so
+//    rounding them costs nothing of the result (see diff_range).
 //  * Partials hold O, its maximum and exp-sum in fp32: the difference of two maps
 //    may be small against either, and a partial rounded to 16 bits, as ordinary
 //    decode keeps it, would cost 2^-8 of the maps.
@@ -33,6 +35,7 @@ namespace {
 
 constexpr int kDiffWaves = 4;  // independent wavefront workers per workgroup
 constexpr int kDiffThreads = kDiffWaves * kWave;
+constexpr int kDiffQueues = 8;       // claim counters of the tiles
 constexpr float kDiffLazyMax = 8.f;  // log2 headroom before a running max moves
 
 // The items of a batch of up to kInlinePlanSeqs, in LDS.
@@ -62,6 +65,9 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   constexpr int NBUF = PF + 1;
   constexpr int EB = KV8 ? 1 : 2;  // pool element bytes
   constexpr int KL = KV8 ? HD / 64 : KK;  // 16-byte key loads of one map
+  // Type of the product with the values: fp8 codes are exact in bf16, whose range
+  // holds a probability times any value scale (fp16's would lose small ones).
+  using PV = Dt<KV8 ? kBF16 : DT>;
 
   const int64_t b0 = vstart(sc, v);
   const int64_t b_end = vstart(sc, v + 1);
@@ -301,14 +307,21 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
         pe[e] = __builtin_amdgcn_exp2f(sc4[e] - mref);
         l_run += pe[e];
       }
-      // The probabilities are rounded to the pool's 16-bit type for the product
-      // (fp8: with the value scale of the half's kv head on them; the exp-sum
-      // takes them unrounded and unscaled).
-      u32x2 pb[2];
+      // The probabilities (fp8: times the value scale of the half's kv head; the
+      // exp-sum takes them unscaled) go into the product as two 16-bit terms,
+      // the rounded value and what the rounding left.  A lane's k-slots of the
+      // 32-deep MFMA are its 4 tokens twice, against the first and the second
+      // terms; the 16-deep one, with rounded probabilities alone, takes as long.
+      // bf16, 64 x 512-4,096 keys, error of the result 2.6e-3 -> 1.7e-3.
+      u32x4 pb[KV8 ? 2 : 1];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const float f = KV8 ? bvs[buf][hf] : 1.f;
-        pb[hf] = u32x2{Dt<DT>::pack2(pe[0] * f, pe[1] * f), Dt<DT>::pack2(pe[2] * f, pe[3] * f)};
+      for (int hf = 0; hf < (KV8 ? 2 : 1); ++hf) {
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = KV8 ? pe[e] * bvs[buf][hf] : pe[e];
+        const uint32_t w0 = PV::pack2(t[0], t[1]), w1 = PV::pack2(t[2], t[3]);
+        pb[hf] = u32x4{w0, w1, PV::pack2(t[0] - PV::lo(w0), t[1] - PV::hi(w0)),
+                       PV::pack2(t[2] - PV::lo(w1), t[3] - PV::hi(w1))};
       }
       // slots past the end may hold anything, NaN bits included: zero their values
       const uint32_t mlo = (kl > 0 ? 0x0000FFFFu : 0u) | (kl > 1 ? 0xFFFF0000u : 0u);
@@ -324,11 +337,11 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
         u32x2 vv;
         if constexpr (KV8) {
           const uint32_t codes = vt[n >> 2][n & 3] & m8;  // a zero code is +0
-          vv = u32x2{Dt<DT>::fp8x2(codes, false), Dt<DT>::fp8x2(codes, true)};
+          vv = u32x2{PV::fp8x2(codes, false), PV::fp8x2(codes, true)};
         } else {
           vv = u32x2{vb[buf][n].x & mlo, vb[buf][n].y & mhi};
         }
-        o[n] = Dt<DT>::mma16x16x16(vv, pb[KV8 ? n / (NT / 2) : 0], o[n]);
+        o[n] = PV::mma16x16x32(u32x4{vv.x, vv.y, vv.x, vv.y}, pb[KV8 ? n / (NT / 2) : 0], o[n]);
       }
     };
 
@@ -472,6 +485,7 @@ template <int DT, int HD, int TPP, bool KV8>
 __global__ __launch_bounds__(kDiffThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void diff_stream_kernel(const DiffParams p) {
   __shared__ DiffPlanLds lds;
+  if (blockIdx.x == 0 && threadIdx.x < kDiffQueues) p.claim[threadIdx.x] = 0;  // for the tiles, the launch behind
   const int64_t n = p.num_seqs;
   const bool lds_plan = n <= kInlinePlanSeqs;
   const int64_t* cum = p.cum;

@@ -704,9 +704,18 @@ int diff_call(const char* op, bool mapped, const void* queries, const void* k_po
   p.head_chunks = (p.group + 7) / 8;
   p.hg_max = hg_max;
   p.num_workers = workers;
+  p.tile_chunks = (p.group + 15) / 16;
+  p.tile_heads = (p.group + p.tile_chunks - 1) / p.tile_chunks;
+  p.tile_magic = (65536u + p.tile_heads - 1) / p.tile_heads;
+  const int64_t tile_rows = 128 / p.tile_heads;
+  const int64_t windows = (num_rows + tile_rows - 1) / tile_rows;
+  if (windows * p.num_kv_heads * p.tile_chunks > 0x7fffffffLL)
+    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] problem too large for one call", op);
+  p.num_windows = static_cast<int>(windows);
   p.scale_log2 = scale_log2_for(head_dim);
   char* ws = static_cast<char*>(workspace);
   p.hdr = reinterpret_cast<int64_t*>(ws);
+  p.claim = reinterpret_cast<uint32_t*>(ws + 128);
   p.cum = reinterpret_cast<int64_t*>(ws + lay.cum);
   p.split_list = reinterpret_cast<int64_t*>(ws + lay.list);
   p.list_cap = workers;

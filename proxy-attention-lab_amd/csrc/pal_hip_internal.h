@@ -175,13 +175,19 @@ hipError_t launch_fused(const DecodeParams& dp, const PrefillParams& pp, int dty
 // neighbouring (page, kv head) blocks), query heads 2i and 2i + 1 the two maps of
 // output head i.  The base's fields keep their meaning with num_kv_heads the
 // number of kv PAIRS, num_q_heads of query heads, group of output heads per kv
-// pair, head_chunks of groups of 8 of them, hg_max = min(group, 8).  Rows as
-// in DecodeParams (row mode: every row, see launch_diff).
+// pair, head_chunks of groups of 8 of them, hg_max = min(group, 8), claim the
+// tiles' 8 counters (the stream kernel clears them).
 struct DiffParams : DecodeParams {
   const float* lambdas;      // [Hq / 2]
   const float* norm_weight;  // [2 HD], or null: no norm
   float norm_eps;
   float out_scale;
+  // tiles of 128 M-rows: tile_heads output heads (at most 16) of tile_chunks groups
+  // per kv pair, num_windows windows of 128 / tile_heads rows
+  int tile_heads;
+  int tile_chunks;
+  int num_windows;
+  uint32_t tile_magic;       // ceil(2^16 / tile_heads): m / tile_heads = m * tile_magic >> 16 for m < 4096
   float* part_o32;           // [virtual workers][2][2 maps][hg_max][2 HD], not normalised (part_ml likewise: max, exp-sum)
 };
 
@@ -189,6 +195,8 @@ struct DiffParams : DecodeParams {
 hipError_t diff_resident_workers(int* workers);
 
 hipError_t launch_diff(const DiffParams& p, int dtype, int head_dim, int tokens_per_page, hipStream_t stream);
+hipError_t launch_diff_bf16(const DiffParams& p, int head_dim, int tokens_per_page, hipStream_t stream);
+hipError_t launch_diff_f16(const DiffParams& p, int head_dim, int tokens_per_page, hipStream_t stream);
 
 // Page moves of a compaction: pages src[m] -> dst[m] of both pools (whole
 // pages, page_bytes each) and, for fp8 pools, their scale rows.  Sources and
@@ -216,6 +224,8 @@ hipError_t decode_debug_flags(uint32_t* out, bool reset);
 hipError_t prefill_debug_flags(uint32_t* out, bool reset);
 hipError_t fill_debug_flags(uint32_t* out, bool reset);
 hipError_t diff_debug_flags(uint32_t* out, bool reset);
+hipError_t diff_bf16_debug_flags(uint32_t* out, bool reset);
+hipError_t diff_f16_debug_flags(uint32_t* out, bool reset);
 
 // Scratch memory held by the library for pal_paged_attention_decode_noalloc:
 // kScratchBytes per device, in a file-scope device array (scratch.hip).

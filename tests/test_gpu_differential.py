@@ -53,6 +53,19 @@ def test_decode_fp8(hd, tpp, dtype):
     run(decode_case(hd + tpp + 1, RAGGED, 16, 4, hd, tpp, dtype, fp8=True), f"decode fp8 hd={hd} tpp={tpp} {dtype}")
 
 
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("factor", [2.0 ** -15, 2.0 ** 9])
+def test_fp8_value_scales(factor, dtype, chunk):
+    """Value scales far from one, on one kv head of the pair or both: neither lost below fp16's range nor past it."""
+    d = chunk_case(60, [300], [(40, 100)], 8, 4, 64, 16, dtype, fp8=True, eps=1e-20, out_scale=0.01) if chunk else \
+        decode_case(60, [300, 20], 8, 4, 64, 16, dtype, fp8=True, eps=1e-20, out_scale=0.01)
+    d.vs *= np.float32(factor)
+    d.vs[:, 3] /= np.float32(factor * 1.37)
+    d.dev["vs"].copy_(torch.from_numpy(d.vs))
+    run(d, f"fp8 value scales x {factor} {dtype} chunk={chunk}")
+
+
 @pytest.mark.parametrize("norm,out_scale", [(True, 1.0), (False, 0.25), (False, 1.0)])
 def test_decode_norm_and_scale(norm, out_scale):
     run(decode_case(3, RAGGED, 8, 4, 64, 16, "f16", norm=norm, out_scale=out_scale), f"decode norm={norm} x {out_scale}")
@@ -100,9 +113,10 @@ def test_decode_lengths_past_the_table_and_extra_rows():
     assert out.shape[0] == 3
 
 
+@pytest.mark.parametrize("norm", [True, False])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_decode_pages_past_the_pool(fp8):
-    d = decode_case(10, [200, 90, 20], 8, 4, 64, 16, "bf16", fp8=fp8)
+def test_decode_pages_past_the_pool(fp8, norm):
+    d = decode_case(10, [200, 90, 20], 8, 4, 64, 16, "bf16", fp8=fp8, norm=norm)
     d.case.page_table[0, 3] = 2 ** 32 - 1
     d.case.page_table[0, 12] = d.case.k_pool.shape[0]
     d.case.page_table[2, :] = d.case.k_pool.shape[0] + 5  # no valid page at all
@@ -259,17 +273,18 @@ def test_any_limits_in_a_run():
     run(Diff(case, q, q2s, off, seed=17), "limits in any order")
 
 
+@pytest.mark.parametrize("norm", [True, False])  # (the norm would hide what changes both maps alike)
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("tpp", [16, 32])
-def test_chunk_pages_past_the_pool(fp8, tpp):
-    d = chunk_case(18, [200], [(150, 100), (0, 64)], 8, 4, 64, tpp, "bf16", fp8=fp8)
+def test_chunk_pages_past_the_pool(fp8, tpp, norm):
+    d = chunk_case(18, [200], [(150, 100), (0, 64)], 8, 4, 64, tpp, "bf16", fp8=fp8, norm=norm)
     pages = d.case.k_pool.shape[0]
     d.case.page_table[0, 2] = pages
     d.case.page_table[1, 1] = 2 ** 32 - 1
     d.case.page_table[1, 5] = pages + 3
     d.case.page_table[2, :] = pages + 9
     d.dev["pt"] = dev_index(d.case.page_table, torch.uint32)
-    run(d, f"chunk, page ids past the pool fp8={fp8}")
+    run(d, f"chunk, page ids past the pool fp8={fp8} norm={norm}")
 
 
 def test_rows_shuffled_in_short_blocks():
