@@ -38,13 +38,176 @@ constexpr int kDiffThreads = kDiffWaves * kWave;
 constexpr int kDiffQueues = 8;       // claim counters of the tiles
 constexpr float kDiffLazyMax = 8.f;  // log2 headroom before a running max moves
 
-// The items of a batch of up to kInlinePlanSeqs, in LDS.
+// Up to kInlinePlanSeqs items of a batch, in LDS.
 struct DiffPlanLds {
   int64_t cum[kInlinePlanSeqs + 1];
   int32_t len[kInlinePlanSeqs];
   int32_t seq[kInlinePlanSeqs];
+  int32_t row[kInlinePlanSeqs];
   int64_t wave_sums[kDiffWaves];
 };
+
+// The plan of a mixed batch's rows, by one workgroup of T threads: the lone rows
+// (alone in their run of rows of one sequence) with keys, and the tiles of the
+// longer runs, each run cut from its first row on.  Tiles are put in order of
+// falling work (the keys of their first row), so that the last ones to start are
+// short: 8 chunks of 512-2,048 rows on 0-2,048 cached, mean end of the workgroups
+// 412 us, last 483 us without.  (A counting sort; equal tiles fall in any order,
+// which changes no result.)  Lone rows without keys get their zeros.
+constexpr int kSortTiles = 4096;     // tiles put in order, at most (more: as they come)
+constexpr int kTileBuckets = 1024;   // of a step of 32 keys, or more for page tables past 32,768 keys
+constexpr int kPlanRows = 16;        // rows of a thread in a sweep
+template <int T>
+struct DiffRowsLds {
+  uint32_t start[kTileBuckets];
+  u32x2 tile[kSortTiles];
+  uint16_t key[kSortTiles];
+  int64_t sums[3][T / kWave];
+  int64_t totals[4];
+};
+template <int T, int kPer, int HD, int TPP>
+__device__ __forceinline__ void diff_plan_rows(const DiffParams& p, DiffRowsLds<T>& L, bool keep_lone) {
+  const int tid = threadIdx.x;
+  const int64_t n = p.num_seqs;
+  const int64_t max_tokens = p.page_table_width * TPP;
+  const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
+  const int per_bucket = max(32, static_cast<int>((max_tokens + kTileBuckets - 1) / kTileBuckets));
+  auto keys_of = [&](uint32_t sq, int64_t r) {
+    if (sq >= p.num_pt_rows) return static_cast<int64_t>(0);
+    const int64_t k = min(p.seq_lens[sq], p.q_offset[r]);
+    PAL_DEBUG_FLAG(k > max_tokens, kDebugLength);
+    return k < 0 ? static_cast<int64_t>(0) : (k > max_tokens ? max_tokens : k);
+  };
+  for (int b = tid; b < kTileBuckets; b += T) L.start[b] = 0;
+  int64_t n_lone = 0, n_blocks = 0, n_tiles = 0, run = 0;  // so far; the first row of the run that a sweep starts in
+  for (int64_t base = 0; base < n; base += static_cast<int64_t>(T) * kPer) {
+    const int64_t r0 = base + static_cast<int64_t>(tid) * kPer;
+    uint32_t sq[kPer + 2];  // sequences of rows r0 - 1 .. r0 + kPer
+#pragma unroll
+    for (int k = 0; k < kPer + 2; ++k) {
+      const int64_t r = r0 - 1 + k;
+      sq[k] = r >= 0 && r < n ? p.q2seq[r] : 0u;
+    }
+    auto starts = [&](int k) { return r0 + k == 0 || sq[k] != sq[k + 1]; };          // row k starts a run
+    auto ends = [&](int k) { return r0 + k + 1 == n || sq[k + 2] != sq[k + 1]; };  // and ends one
+    // the run that row r0 lies in: the last start before it in the sweep, or the run it began in
+    int64_t last = -1;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (r0 + k < n && starts(k)) last = r0 + k;
+    int64_t before = last;  // running maximum over the threads, then of those before this one
+    {
+      const int lane = lane_id();
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int64_t o = __shfl_up(before, off, kWave);
+        if (lane >= off) before = max(before, o);
+      }
+      if (lane == kWave - 1) L.sums[0][tid >> 6] = before;
+      before = __shfl_up(before, 1, kWave);
+      if (lane == 0) before = -1;
+      __syncthreads();
+      for (int i = 0; i < (tid >> 6); ++i) before = max(before, L.sums[0][i]);
+      if (before < 0) before = run;
+      if (tid == T - 1) L.totals[3] = last >= 0 ? last : before;
+      __syncthreads();
+    }
+    // this thread's lone rows and tile starts
+    int64_t lone = 0, blocks = 0, tiles = 0, at = before;
+    uint32_t is_tile = 0;
+    int32_t len[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      len[k] = 0;
+      if (r0 + k >= n) continue;
+      if (starts(k)) at = r0 + k;
+      if (at == r0 + k && ends(k)) {
+        len[k] = static_cast<int32_t>(keys_of(sq[k + 1], r0 + k));
+        if (len[k] > 0) {
+          lone += 1;
+          blocks += ((len[k] + 15) >> 4) * segs;
+        } else if (keep_lone) {
+          zero_item_output<HD>(p, r0 + k);
+        }
+      } else if (static_cast<uint32_t>(r0 + k - at) % static_cast<uint32_t>(p.tile_rows) == 0) {
+        tiles += 1;
+        is_tile |= 1u << k;
+      }
+    }
+    const int64_t lone_to = block_inclusive_scan<T>(lone, L.sums[0]);
+    const int64_t blocks_to = block_inclusive_scan<T>(blocks, L.sums[1]);
+    const int64_t tiles_to = block_inclusive_scan<T>(tiles, L.sums[2]);
+    int64_t li = n_lone + lone_to - lone, bi = n_blocks + blocks_to - blocks, ti = n_tiles + tiles_to - tiles;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (len[k] > 0 && keep_lone) {
+        *reinterpret_cast<u32x4*>(p.lone + 4 * li) =
+            u32x4{static_cast<uint32_t>(r0 + k), sq[k + 1], static_cast<uint32_t>(len[k]), 0u};
+        p.cum[li] = bi;
+        li += 1;
+        bi += ((len[k] + 15) >> 4) * segs;
+      }
+      if (is_tile >> k & 1) {
+        const u32x2 t = {static_cast<uint32_t>(r0 + k), sq[k + 1]};
+        if (ti < kSortTiles) {
+          const int64_t b = keys_of(sq[k + 1], r0 + k) / per_bucket;
+          const int key = kTileBuckets - 1 - static_cast<int>(b < kTileBuckets - 1 ? b : kTileBuckets - 1);
+          L.tile[ti] = t;
+          L.key[ti] = static_cast<uint16_t>(key);
+          atomicAdd(&L.start[key], 1u);
+        } else {
+          *reinterpret_cast<u32x2*>(p.tiles + 2 * ti) = t;
+        }
+        ti += 1;
+      }
+    }
+    if (tid == T - 1) {
+      L.totals[0] = lone_to;
+      L.totals[1] = blocks_to;
+      L.totals[2] = tiles_to;
+    }
+    __syncthreads();
+    n_lone += L.totals[0];
+    n_blocks += L.totals[1];
+    n_tiles += L.totals[2];
+    run = L.totals[3];
+    __syncthreads();
+  }
+  if (tid == 0) {
+    if (keep_lone) {
+      p.hdr[0] = n_blocks;
+      p.hdr[1] = n_lone;
+      p.cum[n_lone] = n_blocks;
+    }
+    p.hdr[2] = n_tiles;
+    p.hdr[3] = n_tiles <= kSortTiles;
+  }
+  if (n_tiles > kSortTiles) {  // too many: in the rows' order
+    for (int i = tid; i < kSortTiles; i += T) *reinterpret_cast<u32x2*>(p.tiles + 2 * i) = L.tile[i];
+    return;
+  }
+  constexpr int kB = kTileBuckets / T;
+  int64_t sum = 0;
+#pragma unroll
+  for (int k = 0; k < kB; ++k) sum += L.start[tid * kB + k];
+  int64_t at = block_inclusive_scan<T>(sum, L.sums[0]) - sum;
+#pragma unroll
+  for (int k = 0; k < kB; ++k) {
+    const uint32_t c = L.start[tid * kB + k];
+    L.start[tid * kB + k] = static_cast<uint32_t>(at);
+    at += c;
+  }
+  __syncthreads();
+  for (int64_t i = tid; i < n_tiles; i += T)
+    *reinterpret_cast<u32x2*>(p.tiles + 2 * atomicAdd(&L.start[L.key[i]], 1u)) = L.tile[i];
+}
+
+// The plan of more rows than a stream workgroup scans.
+template <int HD, int TPP>
+__global__ __launch_bounds__(kPlanThreads) void diff_plan_kernel(const DiffParams p) {
+  __shared__ DiffRowsLds<kPlanThreads> L;
+  diff_plan_rows<kPlanThreads, kPlanRows, HD, TPP>(p, L, true);
+}
 
 // x's value in lane l ^ 8 (a rotation by 8 of each 16 lanes)
 __device__ __forceinline__ float lane_xor8(float x) {
@@ -58,7 +221,7 @@ __device__ __forceinline__ float lane_xor8(float x) {
 // when the piece before it started).
 template <int DT, int HD, int TPP, int PF, bool KV8>
 __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc, const int64_t* cum,
-                                           const DiffPlanLds* plan, int64_t v) {
+                                           const DiffPlanLds* plan, int64_t n_items, int64_t v) {
   static_assert(HD % 32 == 0 && (!KV8 || HD % 64 == 0), "whole k-steps and stripes");
   constexpr int KK = HD / 32;     // QK k-steps of 32 dims of one map
   constexpr int NT = 2 * HD / 16;  // output tiles of 16 dims
@@ -96,25 +259,31 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   const int64_t head_block = static_cast<int64_t>(HD) * TPP * EB;  // bytes per (page, kv head)
   const int64_t page_stride = head_block * 2 * p.num_kv_heads;
 
-  // A piece: item s (of page-table row `seq`, `len` keys, nb blocks per segment),
+  // A piece: item s (row `row` of page-table row `seq`, `len` keys, nb blocks per segment),
   // segment `seg`, blocks [blk, blk + count) of the segment, from global block
   // gpos on; r = block offset of the piece inside the item's segments.  c_* is
   // the piece being computed, x_* the next one (kept in scalars).
-  int64_t c_s, c_r, c_gpos, c_seq, c_len, c_nb, c_blk, c_count;
+  int64_t c_s, c_r, c_gpos, c_row, c_seq, c_len, c_nb, c_blk, c_count;
   int c_seg;
-  int64_t x_s, x_r, x_gpos, x_seq, x_len, x_nb, x_blk, x_count;
+  int64_t x_s, x_r, x_gpos, x_row, x_seq, x_len, x_nb, x_blk, x_count;
   int x_seg;
 #define PAL_FIND_PIECE(P, S0, R0, G0)                                                      \
   do {                                                                                     \
-    int64_t s_ = (S0), r_ = (R0), len_, seq_;                                              \
+    int64_t s_ = (S0), r_ = (R0), len_, seq_, row_;                                        \
     for (;;) {                                                                             \
       if (plan) {                                                                          \
         len_ = plan->len[s_];                                                              \
         seq_ = plan->seq[s_];                                                              \
+        row_ = plan->row[s_];                                                              \
+      } else if (p.q2seq) {                                                                \
+        row_ = p.lone[4 * s_];                                                             \
+        seq_ = p.lone[4 * s_ + 1];                                                         \
+        len_ = p.lone[4 * s_ + 2];                                                         \
       } else {                                                                             \
         const Item it_ = item_at(p, s_, TPP);                                              \
         len_ = it_.len;                                                                    \
         seq_ = it_.seq;                                                                    \
+        row_ = s_;                                                                         \
       }                                                                                    \
       if (len_ > 0) break;                                                                 \
       ++s_;                                                                                \
@@ -123,6 +292,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     P##s = s_;                                                                             \
     P##r = r_;                                                                             \
     P##gpos = (G0);                                                                        \
+    P##row = row_;                                                                         \
     P##seq = seq_;                                                                         \
     P##len = len_;                                                                         \
     P##nb = (len_ + 15) >> 4;                                                              \
@@ -134,12 +304,12 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   // Q^T operand of a piece: the dims of this lane's k-slices of its column's
   // query (zeros in columns without a head).
   u32x4 qv[KK], qn[KK];
-  auto load_q = [&](int64_t s, int seg, u32x4 (&q)[KK]) {
+  auto load_q = [&](int64_t row, int seg, u32x4 (&q)[KK]) {
     const int h0 = (seg % p.head_chunks) * 8;
     const bool hv = r8 < min(8, p.group - h0);
     const uint32_t qmask = hv ? 0xFFFFFFFFu : 0u;
     const int64_t head = static_cast<int64_t>(seg / p.head_chunks) * p.group + h0 + (hv ? r8 : 0);
-    const uint16_t* qrow = p.q + (s * p.num_q_heads + 2 * head + map) * HD;
+    const uint16_t* qrow = p.q + (row * p.num_q_heads + 2 * head + map) * HD;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       if constexpr (KV8)  // k-step kk = (stripe g + 4 (kk / 2), half kk % 2)
@@ -156,10 +326,10 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     return pt[lp];
   };
   {
-    const int64_t s0 = locate_seq(cum, p.num_seqs, b0);  // the item holding block b0 (it has blocks)
+    const int64_t s0 = locate_seq(cum, n_items, b0);  // the item holding block b0 (it has blocks)
     PAL_FIND_PIECE(c_, s0, b0 - cum[s0], b0);
   }
-  load_q(c_s, c_seg, qv);
+  load_q(c_row, c_seg, qv);
 
   // Page ids in register windows of 64 pages: pid_cur holds window wcur, the
   // window of the block being computed, pid_nxt the next one; every step group
@@ -178,7 +348,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   bool first = true;     // the piece is the worker's first
   bool prologue = true;  // the pipeline is empty
   bool has_next = false;
-  x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
+  x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_row = c_row; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
   x_count = c_count; x_seg = c_seg;
   uint32_t pidn0 = 0;        // window 0 of the next piece (a load in flight)
   uint32_t pidn0_ready = 0;  // the same once it has arrived (see below)
@@ -365,10 +535,10 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       if (has_next) {
         PAL_FIND_PIECE(x_, s_n, r_n, gpos_n);
       } else {
-        x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
+        x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_row = c_row; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
         x_count = c_count; x_seg = c_seg;
       }
-      load_q(x_s, x_seg, qn);
+      load_q(x_row, x_seg, qn);
       pidn0 = load_window(x_seq, x_blk, 0);
     }
     const uint32_t pidn1 = load_window(x_seq, x_blk, 1);
@@ -438,7 +608,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       if (p.norm_weight) scale *= 1.f / sqrtf(sum_xor32(sum_xor16(ss)) * (1.f / (2 * HD)) + p.norm_eps);
       if (r8 < hg) {
         // the two lanes of a head write half of its row each
-        uint16_t* row = p.out + (c_s * (p.num_q_heads / 2) + head) * (2 * HD) + 4 * g;
+        uint16_t* row = p.out + (c_row * (p.num_q_heads / 2) + head) * (2 * HD) + 4 * g;
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
           const int t = n + map * (NT / 2);
@@ -459,7 +629,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       if (c_blk == 0) {  // the first piece of a split segment ends the worker's range
         list_g0 = c_gpos;
         list_nb = c_nb;
-        list_row = c_s;
+        list_row = c_row;
         list_seg = c_seg;
       }
     }
@@ -468,7 +638,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     if (!has_next) break;
     // the next piece becomes current: its first PF blocks are in flight, in
     // buffers 0 .. PF-1 (n_pad is a multiple of NBUF)
-    c_s = x_s; c_r = x_r; c_gpos = x_gpos; c_seq = x_seq; c_len = x_len; c_nb = x_nb; c_blk = x_blk;
+    c_s = x_s; c_r = x_r; c_gpos = x_gpos; c_row = x_row; c_seq = x_seq; c_len = x_len; c_nb = x_nb; c_blk = x_blk;
     c_count = x_count; c_seg = x_seg;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qv[kk] = qn[kk];
@@ -484,17 +654,26 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
 template <int DT, int HD, int TPP, bool KV8>
 __global__ __launch_bounds__(kDiffThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void diff_stream_kernel(const DiffParams p) {
-  __shared__ DiffPlanLds lds;
-  if (blockIdx.x == 0 && threadIdx.x < kDiffQueues) p.claim[threadIdx.x] = 0;  // for the tiles, the launch behind
+  __shared__ union {
+    DiffPlanLds plan;
+    DiffRowsLds<kDiffThreads> rows;
+  } lds_all;
+  DiffPlanLds& lds = lds_all.plan;
   const int64_t n = p.num_seqs;
-  const bool lds_plan = n <= kInlinePlanSeqs;
+  const int tid = threadIdx.x;
+  const bool scan = n <= kInlinePlanSeqs;
+  constexpr int kPer = kInlinePlanSeqs / kDiffThreads;
+  if (p.q2seq && scan && blockIdx.x + 1 == gridDim.x) {  // the workgroup behind the workers'
+    diff_plan_rows<kDiffThreads, kPer, HD, TPP>(p, lds_all.rows, false);
+    return;
+  }
+  if (blockIdx.x == 0 && tid < kDiffQueues) p.claim[tid] = 0;  // for the tiles, the launch behind
+  int64_t n_items = n, total;
   const int64_t* cum = p.cum;
-  int64_t total;
-  if (lds_plan) {
+  const DiffPlanLds* plan = nullptr;
+  if (scan) {
     // every workgroup scans the lengths into LDS: thread t owns items 4t .. 4t+3
-    constexpr int kPer = kInlinePlanSeqs / kDiffThreads;
     const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
-    const int tid = threadIdx.x;
     int64_t vals[kPer];
     int64_t tsum = 0;
 #pragma unroll
@@ -506,6 +685,7 @@ void diff_stream_kernel(const DiffParams p) {
         vals[k] = ((it.len + 15) >> 4) * segs;
         lds.len[s] = static_cast<int32_t>(it.len);
         lds.seq[s] = static_cast<int32_t>(it.seq);
+        lds.row[s] = static_cast<int32_t>(s);
         if (it.len == 0 && !it.skip && blockIdx.x == 0) zero_item_output<HD>(p, it.row);
       }
       tsum += vals[k];
@@ -522,14 +702,29 @@ void diff_stream_kernel(const DiffParams p) {
     __syncthreads();
     total = lds.cum[n];
     if (blockIdx.x == 0 && tid == 0) p.hdr[0] = total;
-    cum = lds.cum;
+    plan = &lds;
   } else {
     total = p.hdr[0];
+    if (p.q2seq) {  // the lone rows that the plan found
+      n_items = p.hdr[1];
+      if (total > 0 && n_items <= kInlinePlanSeqs) {
+        for (int64_t s = tid; s < n_items; s += kDiffThreads) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(p.lone + 4 * s);
+          lds.row[s] = static_cast<int32_t>(v.x);
+          lds.seq[s] = static_cast<int32_t>(v.y);
+          lds.len[s] = static_cast<int32_t>(v.z);
+          lds.cum[s] = p.cum[s];
+        }
+        __syncthreads();
+        plan = &lds;
+      }
+    }
   }
+  if (plan) cum = plan->cum;
   if (total == 0) return;
   const Sched sc = make_sched(total, p.num_workers, 0);
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kDiffWaves + wave_id();
-  if (w < sc.nws) diff_range<DT, HD, TPP, KV8 ? 3 : 2, KV8>(p, sc, cum, lds_plan ? &lds : nullptr, w);
+  if (w < sc.nws) diff_range<DT, HD, TPP, KV8 ? 3 : 2, KV8>(p, sc, cum, plan, n_items, w);
 }
 
 // Joins the pieces of split segments: workgroup (v, h) takes head h of the

@@ -11,20 +11,25 @@ namespace {
 
 template <int DT, int HD, int TPP, bool KV8>
 hipError_t launch_diff_t(const DiffParams& p, hipStream_t stream) {
-  if (p.num_seqs > kInlinePlanSeqs) {
-    hipLaunchKernelGGL((decode_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
+  const bool inline_plan = p.num_seqs <= kInlinePlanSeqs;
+  if (!inline_plan) {
+    if (p.q2seq)
+      hipLaunchKernelGGL((diff_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  hipLaunchKernelGGL((diff_stream_kernel<DT, HD, TPP, KV8>), dim3(static_cast<unsigned>(p.num_workers / kDiffWaves)),
-                     dim3(kDiffThreads), 0, stream, p);
+  hipLaunchKernelGGL((diff_stream_kernel<DT, HD, TPP, KV8>),
+                     dim3(static_cast<unsigned>(p.num_workers / kDiffWaves + (p.q2seq && inline_plan ? 1 : 0))), dim3(kDiffThreads), 0,
+                     stream, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL((diff_merge_kernel<DT, HD>), dim3(static_cast<unsigned>(p.num_workers), static_cast<unsigned>(p.hg_max)),
                      dim3(kDiffThreads), 0, stream, p);
   err = hipGetLastError();
   if (err != hipSuccess || !p.q2seq) return err;
-  const int64_t items = p.num_windows * static_cast<int64_t>(p.num_kv_heads) * p.tile_chunks;
+  const int64_t items = (p.num_seqs / 2 + 1) * p.num_kv_heads * p.tile_chunks;  // at most
   const int64_t cus = p.num_workers / kDiffWaves;
   hipLaunchKernelGGL((diff_tile_kernel<DT, HD, TPP, KV8>), dim3(static_cast<unsigned>(items < cus ? items : cus)),
                      dim3(kPfThreads), sizeof(DiffTileLds<HD, KV8>), stream, p);

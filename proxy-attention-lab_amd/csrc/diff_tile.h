@@ -106,6 +106,25 @@ __device__ __forceinline__ float diff_acc_get() {
   else asm volatile("v_accvgpr_read_b32 %0, a[%1]" : "=v"(v) : "n"(kDiffAcc + X - 128));
   return v;
 }
+// element X times f
+template <int X>
+__device__ __forceinline__ float diff_acc_mul(float f) {
+  if constexpr (X < 128) {
+    float v;
+    asm volatile("v_mul_f32 %0, v[%1], %2" : "=v"(v) : "n"(kDiffAcc + X), "v"(f));
+    return v;
+  } else {
+    return diff_acc_get<X>() * f;
+  }
+}
+// element X (of the VGPRs) = itself times f plus t; ss += its square
+template <int X>
+__device__ __forceinline__ void diff_acc_join(float f, float t, float& ss) {
+  static_assert(X < 128, "an accumulator in VGPRs");
+  asm volatile("v_fma_f32 v[%1], v[%1], %2, %3\n\tv_fma_f32 %0, v[%1], v[%1], %0"
+               : "+v"(ss)
+               : "n"(kDiffAcc + X), "v"(f), "v"(t));
+}
 template <int X>
 __device__ __forceinline__ void diff_acc_put(float v) {
   if constexpr (X < 128) asm volatile("v_mov_b32 v[%1], %0" ::"v"(v), "n"(kDiffAcc + X));
@@ -122,6 +141,16 @@ __device__ __forceinline__ DiffArgs* diff_args() {
   DiffArgs* a = (DiffArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(a));
   return a;
+}
+
+// The lane, computed here and now: what is derived from the kernel's thread index
+// the compiler computes once, before all tiles, and spills, and reading it back
+// from scratch memory waits for every copy and store in flight (the output of a
+// tile took 9.3 us of that).
+__device__ __forceinline__ int lane_now() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
 }
 
 // Steps of K (and of V): the 16-byte items of the pair's block
@@ -141,18 +170,15 @@ struct DiffTileLds {
   uint32_t pid[2 * kPidChunk];
   float scl[KV8 ? 8 * kPidChunk : 1];  // fp8: scales of each staged page id, [K1, K2, V1, V2][slot]
   int lim[kDiffMRows + 2 * kPfWaves + 1];
-  uint32_t seq[kDiffMRows];
-  int32_t off[kDiffMRows];
-  uint64_t start[kDiffMRows / kWave];  // rows that start a run, rows alone in their run
-  uint64_t lone[kDiffMRows / kWave];
+  uint64_t other[kDiffMRows / kWave];  // rows of another sequence than the tile's
   uint32_t next[2];
-  int win[8];  // the window: first row, rows, kv pair, first head, heads, item, claim queue
-  int run[2];  // the running tile's rows [run[0], run[1]) of the window
+  int tile[8];  // the tile: first row, rows, kv pair, first head, heads, claim queue
+  __attribute__((aligned(16))) float weight[2 * HD];  // what a row is scaled with behind its norm
 };
 
-// One query tile: rows [at, end) of the window in L, a run of one sequence's rows.
+// Item `item`: head group item % G (G = kv pairs x head chunks) of tile item / G.
 template <int DT, int HD, int TPP, bool KV8>
-__device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>& L) {
+__device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTileLds<HD, KV8>& L) {
   constexpr int VD = 2 * HD;
   constexpr int KS = HD / 16;  // QK k-steps of a map; also row tiles of 32 value dims
   constexpr int NQ = 2 * KS;   // QK MFMAs of a step (and PV operands, two MFMAs each)
@@ -163,20 +189,25 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   using IM = ItemMap<VD, TPP>;
   auto k_lds = [&](int j) { return L.k + (j & (kNBuf - 1)) * NI * 8; };  // step j's buffer
   auto v_lds = [&](int j) { return L.v + (j & (kNBuf - 1)) * NI * 8; };
-
   auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int row0 = uniform(L.win[0]) + at;
-  const int nrows = end - at;
-  const int pair = uniform(L.win[2]), h0 = uniform(L.win[3]), hg = uniform(L.win[4]);
+
   DiffArgs* args = diff_args();
-  const uint32_t seq_u = uniform(static_cast<int>(L.seq[at]));
+  const unsigned G = static_cast<unsigned>(args->num_kv_heads) * args->tile_chunks;
+  const unsigned index = item / G;
+  const unsigned grp = item - index * G;
+  const uint32_t* entry = args->tiles + 2 * (args->hdr[3] ? index : static_cast<unsigned>(args->hdr[2]) - 1 - index);
+  const int row0 = uniform(static_cast<int>(entry[0]));
+  const uint32_t seq_u = static_cast<uint32_t>(uniform(static_cast<int>(entry[1])));
+  const int tile_heads = args->tile_heads;
+  const int pair = static_cast<int>(grp / args->tile_chunks);
+  const int h0 = static_cast<int>(grp % args->tile_chunks) * tile_heads;
+  const int hg = min(tile_heads, args->group - h0);
   const bool seq_ok = seq_u < args->num_pt_rows;  // a row naming no sequence attends to nothing
   const int64_t s = seq_ok ? seq_u : 0;
-  const int tile_heads = args->tile_heads;
-  const int qt = kDiffMRows / tile_heads;  // tokens per tile
-  const int tid = threadIdx.x;
-  const int lane = lane_id();
+  const int qt = args->tile_rows;  // tokens per tile
+  const int lane = lane_now();
   const int w = wave_id();
+  const int tid = w * kWave + lane;
   const int col = lane & 31;  // this lane's M-row within the wavefront's
   const int half = lane >> 5;
 
@@ -185,10 +216,14 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   PAL_DEBUG_FLAG(slen > max_tokens, kDebugLength);
   slen = slen < 0 ? 0 : (slen > max_tokens ? max_tokens : slen);
 
-  // loads that need only the tile's coordinates: queries, first page-table entries
+  // The loads that need only the tile's coordinates: its rows' sequences and key
+  // limits, first page-table entries, queries.  (Rows past the tile's run are found
+  // out below; they may be read as if they were the tile's.)
   constexpr int kBad = kDiffMRows + 2 * kPfWaves;  // L.lim word set when a staged page id is out of range
-  const bool live_tok = tid < nrows && tid < qt;
-  const int tok_off = live_tok ? L.off[at + tid] : 0;
+  const int64_t n_rows = args->num_seqs;
+  const bool in = tid < qt && row0 + tid < n_rows;
+  const uint32_t row_seq = in ? args->q2seq[row0 + tid] : ~seq_u;
+  const int tok_off = in ? args->q_offset[row0 + tid] : 0;
   const uint32_t* pt0 = args->page_table + s * args->page_table_width;
   constexpr int kPidPre = kPidChunk / kPfThreads;
   uint32_t pid_pre[kPidPre];
@@ -200,38 +235,58 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   const int m_row = w * 32 + col;
   const int my_t = static_cast<int>((static_cast<uint32_t>(m_row) * args->tile_magic) >> 16);  // m_row / tile_heads
   const int my_h = m_row - my_t * tile_heads;
-  const bool row_ok = my_t < nrows && my_t < qt && my_h < hg;
-  const int head = pair * args->group + h0 + (row_ok ? my_h : 0);
+  const bool may = my_t < qt && row0 + my_t < n_rows && my_h < hg;
+  const int head = pair * args->group + h0 + (may ? my_h : 0);
   // Q^T operands of both maps: Q[M-row col][16 kk + 8 half .. +7] (an M-row past
   // the tile takes the first's; its result is not written); fp8 steps: k-step
   // 2j + e takes dims 16 (2j + half) + 8e .. +7, as the key items hold them
   u32x4 qv[2][KS];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const uint16_t* qp = args->q + (static_cast<int64_t>(row0 + (row_ok ? my_t : 0)) * args->num_q_heads + 2 * head + r) * HD;
+    const uint16_t* qp = args->q + (static_cast<int64_t>(row0 + (may ? my_t : 0)) * args->num_q_heads + 2 * head + r) * HD;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk)
       qv[r][kk] = *reinterpret_cast<const u32x4*>(qp + (F8 ? 32 * (kk / 2) + 16 * half + 8 * (kk % 2) : 16 * kk + 8 * half));
   }
   __syncthreads();  // the previous tile is done with every LDS array
-  if (tid == 0) {
-    L.run[0] = at;
-    L.run[1] = end;
+  if (tid < VD) L.weight[tid] = args->out_scale * (args->norm_weight ? args->norm_weight[tid] : 1.f);
+  if (w < kDiffMRows / kWave) {
+    const uint64_t m = __ballot(row_seq != seq_u);
+    if (lane == 0) L.other[w] = m;
   }
+  __syncthreads();
+  // rows of the tile: up to the first of another sequence (or the last of the call)
+  int nrows = qt;
+#pragma unroll
+  for (int i = kDiffMRows / kWave - 1; i >= 0; --i) {
+    const uint64_t m = (static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(L.other[i] >> 32)))) << 32) |
+                       static_cast<uint32_t>(uniform(static_cast<int>(L.other[i])));
+    if (m) nrows = min(qt, i * kWave + static_cast<int>(__builtin_ctzll(m)));
+  }
+  const bool row_ok = may && my_t < nrows;
   {
+    const bool live = tid < nrows;
     int lim = 0;
-    if (live_tok) {
+    if (live) {
       const int64_t off = tok_off < 0 ? 0 : tok_off;
       lim = static_cast<int>(off < slen ? off : slen);
     }
     if (tid < kDiffMRows) L.lim[tid] = lim;
     const int mx = wave_max(lim);
-    const int mn = -wave_max(live_tok ? -lim : -(1 << 30));
+    const int mn = -wave_max(live ? -lim : -(1 << 30));
     if (lane == 0) {
       L.lim[kDiffMRows + w] = mx;
       L.lim[kDiffMRows + kPfWaves + w] = mn;
     }
-    if (tid == 0) L.lim[kBad] = 0;
+    if (tid == 0) {
+      L.lim[kBad] = 0;
+      L.tile[0] = row0;
+      L.tile[1] = nrows;
+      L.tile[2] = pair;
+      L.tile[3] = h0;
+      L.tile[4] = hg;
+      L.tile[5] = static_cast<int>(queue);
+    }
   }
   __syncthreads();
   int max_lim = 0, min_lim = 1 << 30;
@@ -257,7 +312,7 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
     const bool ok = pg < a0->num_pages;
     if (!ok) L.lim[kBad] = 1;
     if constexpr (F8) {  // (0 for an invalid id: such a step's codes are zeros)
-      const int64_t si = 2 * (static_cast<int64_t>(ok ? pg : 0) * a0->num_kv_heads + uniform(L.win[2]));
+      const int64_t si = 2 * (static_cast<int64_t>(ok ? pg : 0) * a0->num_kv_heads + uniform(L.tile[2]));
 #pragma unroll
       for (int a = 0; a < 4; ++a)
         L.scl[a * 2 * kPidChunk + pid_slot(e)] = ok ? (a < 2 ? a0->k_scales : a0->v_scales)[si + (a & 1)] : 0.f;
@@ -266,7 +321,8 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   auto stage_pids = [&](int chunk) {  // synchronous; callers hold a barrier after it
     DiffArgs* a = diff_args();
     const uint32_t* pt = a->page_table + s * a->page_table_width;
-    for (int e = chunk * kPidChunk + tid; e < min((chunk + 1) * kPidChunk, n_pid); e += kPfThreads) stage_pid(a, e, pt[e]);
+    for (int e = chunk * kPidChunk + w * kWave + lane_now(); e < min((chunk + 1) * kPidChunk, n_pid); e += kPfThreads)
+      stage_pid(a, e, pt[e]);
   };
 
   // Items of a step (see prefill_tile.h; the pair's block as one of VD dims).
@@ -291,7 +347,6 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
     d = i % VD;
     kb = 16 * (i / VD);
   };
-  auto item_of = [&](int q) { return tid + q * kPfThreads; };
   auto wave_item = [&](int q) { return w * kWave + q * kPfThreads; };
   auto live_copy = [&](int q) { return kAllItems || wave_item(q) < NI; };
   const uint64_t k_pair = reinterpret_cast<uint64_t>(args->k_pool) + pair * pair_block * (F8 ? 1 : 2);
@@ -346,10 +401,11 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
     uint16_t* kb = k_lds(j);
     DiffArgs* a = diff_args();
     const int64_t stride = pair_block * a->num_kv_heads * (F8 ? 1 : 2);  // bytes of a page
-    const uint64_t from = reinterpret_cast<uint64_t>(a->k_pool) + uniform(L.win[2]) * pair_block * (F8 ? 1 : 2);
-#pragma unroll
+    const uint64_t from = reinterpret_cast<uint64_t>(a->k_pool) + uniform(L.tile[2]) * pair_block * (F8 ? 1 : 2);
+    const int first = w * kWave + lane_now();
+#pragma unroll 1
     for (int q = 0; q < NC; ++q) {
-      const int i = item_of(q);
+      const int i = first + q * kPfThreads;
       if (i >= NI) continue;
       int ph, c, key;
       if constexpr (F8) {
@@ -394,10 +450,11 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
     uint16_t* vb = v_lds(j);
     DiffArgs* a = diff_args();
     const int64_t stride = pair_block * a->num_kv_heads * (F8 ? 1 : 2);
-    const uint64_t from = reinterpret_cast<uint64_t>(a->v_pool) + uniform(L.win[2]) * pair_block * (F8 ? 1 : 2);
-#pragma unroll
+    const uint64_t from = reinterpret_cast<uint64_t>(a->v_pool) + uniform(L.tile[2]) * pair_block * (F8 ? 1 : 2);
+    const int first = w * kWave + lane_now();
+#pragma unroll 1
     for (int q = 0; q < NC; ++q) {
-      const int i = item_of(q);
+      const int i = first + q * kPfThreads;
       if (i >= NI) continue;
       int ph, d, key;
       v_place(i, ph, d, key);
@@ -417,9 +474,10 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
     __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
     compiler_fence();
     uint16_t* vb = v_lds(j);
-#pragma unroll
+    const int first = w * kWave + lane_now();
+#pragma unroll 1
     for (int q = 0; q < NC; ++q) {
-      const int i = item_of(q);
+      const int i = first + q * kPfThreads;
       if (i >= NI) continue;
       int ph, d, key;
       v_place(i, ph, d, key);
@@ -553,7 +611,7 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   // of K read in the PV half and all of V in the QK half, the LDS would be
   // asked for its whole rate in the latter, and twice the registers hold
   // operands.
-  constexpr int kAhead = HD == 128 ? 10 : (HD == 96 ? 8 : NQ);
+  constexpr int kAhead = HD == 128 ? 8 : (HD == 96 ? 8 : NQ);
   Op ka[NQ];
   const int paged_full = !long_pages ? max_lim / kKeys : 0;  // whole steps
   if (nsteps > 0) {
@@ -848,19 +906,18 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   // leave through LDS (the step buffers; 16-byte chunk c of row i at chunk c ^ i)
   // as whole rows.
   DiffArgs* out_args = diff_args();
-  const float* norm_weight = out_args->norm_weight;
+  const int out_lane = lane_now(), out_col = out_lane & 31, out_half = out_lane >> 5;
   const float l1 = sum_xor32(l_run[0]), l2 = sum_xor32(l_run[1]);
   const float f1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f;  // (no score above -inf: the map adds nothing)
   const float f2 = l2 > 0.f || l2 != l2 ? -out_args->lambdas[head] / l2 : 0.f;
-  float ss = 0.f;
+  float ss[4] = {0.f, 0.f, 0.f, 0.f};
   static_for<KS * 16>([&](auto xc) {
     constexpr int X = decltype(xc)::value;
-    const float x = diff_acc_get<X>() * f1 + diff_acc_get<KS * 16 + X>() * f2;
-    diff_acc_put<X>(x);
-    ss += x * x;
+    diff_acc_join<X>(f1, diff_acc_mul<KS * 16 + X>(f2), ss[X % 4]);
   });
-  float scale = out_args->out_scale;
-  if (norm_weight) scale *= 1.f / sqrtf(sum_xor32(ss) * (1.f / VD) + out_args->norm_eps);
+  float scale = 1.f;
+  if (out_args->norm_weight)
+    scale = 1.f / sqrtf(sum_xor32((ss[0] + ss[1]) + (ss[2] + ss[3])) * (1.f / VD) + out_args->norm_eps);
   __syncthreads();  // every wavefront has read the last step
   constexpr int kCh = VD / 8;  // 16-byte chunks of a row
   auto place_chunk = [](int row, int c) { return (kCh & (kCh - 1)) == 0 ? c ^ (row & (kCh - 1)) : (c + row) % kCh; };
@@ -869,106 +926,29 @@ __device__ __forceinline__ void diff_tile(int at, int end, DiffTileLds<HD, KV8>&
   static_for<KS * 4>([&](auto qc) {
     constexpr int c = decltype(qc)::value;  // dims 8c + 4 half .. +3
     constexpr int x = 16 * (c / 4) + 4 * (c % 4);
-    f32x4 y = {diff_acc_get<x>(), diff_acc_get<x + 1>(), diff_acc_get<x + 2>(), diff_acc_get<x + 3>()};
-    y *= scale;
-    if (norm_weight) y *= *reinterpret_cast<const f32x4*>(norm_weight + 8 * c + 4 * half);
-    *reinterpret_cast<u32x2*>(region + col * VD + place_chunk(col, c) * 8 + 4 * half) =
-        u32x2{Dt<DT>::pack2(y[0], y[1]), Dt<DT>::pack2(y[2], y[3])};
+    const f32x4 wt = *reinterpret_cast<const f32x4*>(L.weight + 8 * c + 4 * out_half);
+    const float y0 = diff_acc_mul<x>(scale) * wt[0], y1 = diff_acc_mul<x + 1>(scale) * wt[1];
+    const float y2 = diff_acc_mul<x + 2>(scale) * wt[2], y3 = diff_acc_mul<x + 3>(scale) * wt[3];
+    *reinterpret_cast<u32x2*>(region + out_col * VD + place_chunk(out_col, c) * 8 + 4 * out_half) =
+        u32x2{Dt<DT>::pack2(y0, y1), Dt<DT>::pack2(y2, y3)};
   });
   compiler_fence();
   __builtin_amdgcn_s_waitcnt(kLgkmZero);  // a wavefront reads only what it wrote
   compiler_fence();
-  const int out_tile_heads = out_args->tile_heads, out_heads = out_args->num_q_heads / 2, out_qt = kDiffMRows / out_tile_heads;
-  const int out_at = uniform(L.run[0]), out_rows = uniform(L.run[1]) - out_at, out_hg = uniform(L.win[4]);
-  uint16_t* out_tile = out_args->out + (static_cast<int64_t>(uniform(L.win[0]) + out_at) * out_heads + uniform(L.win[2]) * out_args->group +
-                                        uniform(L.win[3])) * VD;
+  const int out_tile_heads = out_args->tile_heads, out_heads = out_args->num_q_heads / 2, out_qt = out_args->tile_rows;
+  const int out_rows = uniform(L.tile[1]), out_hg = uniform(L.tile[4]);
+  uint16_t* out_tile = out_args->out + (static_cast<int64_t>(uniform(L.tile[0])) * out_heads + uniform(L.tile[2]) * out_args->group +
+                                        uniform(L.tile[3])) * VD;
 #pragma unroll
   for (int it = 0; it < kCh / 2; ++it) {
-    const int i = it * kWave + lane;
+    const int i = it * kWave + out_lane;
     const int row = i / kCh, c = i % kCh;
     const int m = w * 32 + row;
     const int t = static_cast<int>((static_cast<uint32_t>(m) * out_args->tile_magic) >> 16);
     const int h = m - t * out_tile_heads;
     const u32x4 val = *reinterpret_cast<const u32x4*>(region + row * VD + place_chunk(row, c) * 8);
     if (t < out_rows && t < out_qt && h < out_hg)
-      __builtin_nontemporal_store(
-          val, reinterpret_cast<u32x4*>(out_tile + (static_cast<int64_t>(t) * out_heads + h) * VD + c * 8));
-  }
-}
-
-// Item `item`: head group item % G (G = kv pairs x head chunks), window item / G
-// from the last on (later rows of a sequence usually see more keys).  Every run
-// of rows of one sequence in the window that is not a lone row is a tile.
-template <int DT, int HD, int TPP, bool KV8>
-__device__ __forceinline__ void diff_window(unsigned item, uint32_t queue, DiffTileLds<HD, KV8>& L) {
-  constexpr int kMasks = kDiffMRows / kWave;
-  {
-    DiffArgs* p = diff_args();
-    const unsigned G = static_cast<unsigned>(p->num_kv_heads) * p->tile_chunks;
-    const int grp = static_cast<int>(item % G);
-    const int unit = static_cast<int>(item / G);
-    const int h0 = (grp % p->tile_chunks) * p->tile_heads;
-    const int qt = kDiffMRows / p->tile_heads;
-    const int64_t w0 = static_cast<int64_t>(p->num_windows - 1 - unit) * qt;
-    const int n = static_cast<int>(min(static_cast<int64_t>(qt), p->num_seqs - w0));
-    const int i = threadIdx.x;
-    const bool in = i < n;
-    const int64_t r = w0 + i;
-    uint32_t cur = 0, prev = 0, next = 0;
-    int32_t off = 0;
-    if (in) {
-      cur = p->q2seq[r];
-      prev = r > 0 ? p->q2seq[r - 1] : 0u;
-      next = r + 1 < p->num_seqs ? p->q2seq[r + 1] : 0u;
-      off = p->q_offset[r];
-    }
-    __syncthreads();  // the previous item is done with the window
-    if (wave_id() < kMasks) {
-      const bool head = in && (r == 0 || prev != cur);  // starts a run of its sequence's rows
-      const bool tail = in && (r + 1 == p->num_seqs || next != cur);
-      L.seq[i] = cur;
-      L.off[i] = off;
-      const uint64_t st = __ballot(in && (i == 0 || head));
-      const uint64_t lo = __ballot(head && tail);
-      if (lane_id() == 0) {
-        L.start[wave_id()] = st;
-        L.lone[wave_id()] = lo;
-      }
-    }
-    if (threadIdx.x == 0) {
-      L.win[0] = static_cast<int>(w0);
-      L.win[1] = n;
-      L.win[2] = grp / p->tile_chunks;
-      L.win[3] = h0;
-      L.win[4] = min(p->tile_heads, p->group - h0);
-      L.win[5] = static_cast<int>(item);
-      L.win[6] = static_cast<int>(queue);
-    }
-  }
-  __syncthreads();
-  auto uniform64 = [](uint64_t v) {
-    return (static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32) |
-           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
-  };
-  int at = 0;
-  for (;;) {
-    const int n = __builtin_amdgcn_readfirstlane(L.win[1]);
-    if (at >= n) return;
-    int end = n;  // the next run's start, from the masks' bits past `at`
-    for (int b = (at + 1) / kWave; b < kMasks; ++b) {
-      uint64_t m = uniform64(L.start[b]);
-      if (b == (at + 1) / kWave) m &= ~0ull << ((at + 1) % kWave);
-      if (m) {
-        end = min(n, b * kWave + static_cast<int>(__builtin_ctzll(m)));
-        break;
-      }
-    }
-    if ((uniform64(L.lone[at / kWave]) >> (at % kWave)) & 1) {  // a lone row: streamed
-      at = end;
-      continue;
-    }
-    diff_tile<DT, HD, TPP, KV8>(at, end, L);
-    at = __builtin_amdgcn_readfirstlane(L.run[1]);
+      *reinterpret_cast<u32x4*>(out_tile + (static_cast<int64_t>(t) * out_heads + h) * VD + c * 8) = val;
   }
 }
 
@@ -977,17 +957,21 @@ __global__ __launch_bounds__(kPfThreads) PAL_DIFF_TILE_KERNEL void diff_tile_ker
   extern __shared__ __attribute__((aligned(16))) uint8_t tile_lds[];
   DiffTileLds<HD, KV8>& L = *reinterpret_cast<DiffTileLds<HD, KV8>*>(tile_lds);
   uint32_t queue = blockIdx.x % kDiffQueues;
-  unsigned item = blockIdx.x;  // (the grid has no more workgroups than there are items)
+  unsigned item = blockIdx.x;
   for (;;) {
-    diff_window<DT, HD, TPP, KV8>(item, queue, L);
+    {
+      DiffArgs* p = diff_args();
+      if (item >= static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks) return;
+    }
+    diff_tile<DT, HD, TPP, KV8>(item, queue, L);
     DiffArgs* p = diff_args();
     const unsigned nb = gridDim.x;
-    const unsigned items = static_cast<unsigned>(p->num_windows) * p->num_kv_heads * p->tile_chunks;
+    const unsigned items = static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks;
     if (items <= nb) return;
     // queue q: items q, q + 8, ...; its first ceil((nb - q) / 8) are taken by place
     auto item_of = [&](uint32_t q, uint32_t n) { return q + kDiffQueues * (n + (nb + kDiffQueues - 1 - q) / kDiffQueues); };
     if (threadIdx.x == 0) {
-      uint32_t q = L.win[6];
+      uint32_t q = L.tile[5];
       unsigned next = item_of(q, atomicAdd(p->claim + q, 1u));
       for (int k = 1; k < kDiffQueues && next >= items; ++k) {  // that queue is empty: the next one with an item
         q = (q + 1) % kDiffQueues;
@@ -999,7 +983,6 @@ __global__ __launch_bounds__(kPfThreads) PAL_DIFF_TILE_KERNEL void diff_tile_ker
     __syncthreads();
     item = __builtin_amdgcn_readfirstlane(L.next[0]);
     queue = __builtin_amdgcn_readfirstlane(L.next[1]);
-    if (item >= items) return;
   }
 }
 

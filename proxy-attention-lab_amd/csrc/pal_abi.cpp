@@ -8,42 +8,11 @@
 // memory.
 #include <hip/hip_runtime.h>
 
-#include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <string>
 
-#include "../../include/pal_hip.h"
-#include "pal_hip_internal.h"
-#include "pal_log.h"
+#include "pal_abi_util.h"
 
 namespace {
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  pal::set_last_error(buf);
-  return code;
-}
-
-int ok() {
-  pal::clear_last_error();
-  return PAL_OK;
-}
-
-int hip_status(hipError_t err, const char* what) {
-  if (err == hipSuccess) return ok();
-  return fail(PAL_ERR_HIP, "[%s] HIP error: %s", what, hipGetErrorString(err));
-}
-
-bool valid_dtype(int dtype) { return dtype == PAL_DTYPE_FLOAT16 || dtype == PAL_DTYPE_BFLOAT16; }
-bool valid_pool_dtype(int dtype) { return valid_dtype(dtype) || dtype == PAL_DTYPE_FP8_E4M3; }
-int pool_elem_bytes(int dtype) { return dtype == PAL_DTYPE_FP8_E4M3 ? 1 : 2; }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 bool decode_head_dim_supported(int hd) {
   return hd == 32 || hd == 64 || hd == 80 || hd == 96 || hd == 128 || hd == 256;
@@ -51,17 +20,9 @@ bool decode_head_dim_supported(int hd) {
 
 bool prefill_head_dim_supported(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
-float scale_log2_for(int head_dim) {
-  return static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_dim)));
-}
-
 bool decode_partition_ok(int partition_size) {
   return partition_size == 0 || partition_size == 128 || partition_size == 256 || partition_size == 512;
 }
-
-size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
-constexpr int kMaxPageSize = 1024;  // prefill's run-time page sizes (multiples of 8)
 
 // Decode workspace layout (all offsets 256-aligned).  The 4-byte claim word at
 // byte 64 must be zero when a call starts; every call leaves it zero.  Every
@@ -150,26 +111,6 @@ pal::DecodeParams decode_params(const void* queries, const void* k_pool, const v
   p.tokens_per_worker = partition_size;
   p.scale_log2 = scale_log2_for(head_dim);
   return p;
-}
-
-// Checks shared by every attention entry point; returns PAL_OK or an error.
-int check_attention_dims(const char* op, int dtype, int num_q_heads, int num_kv_heads, int head_dim,
-                         int tokens_per_page, int64_t num_pages, int64_t page_table_width, bool any_page_size = false) {
-  if (!valid_dtype(dtype)) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] unsupported dtype code %d", op, dtype);
-  if (num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || tokens_per_page <= 0 || num_pages < 0 ||
-      page_table_width < 0)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] negative or zero dimension", op);
-  if (num_q_heads % num_kv_heads != 0)
-    return fail(PAL_ERR_RUNTIME, "num_q_heads must be divisible by num_kv_heads (%d %% %d != 0)", num_q_heads,
-                num_kv_heads);
-  if (any_page_size) {  // prefill over 16-bit pools: any multiple of 8 up to kMaxPageSize
-    if (tokens_per_page % 8 != 0 || tokens_per_page > kMaxPageSize)
-      return fail(PAL_ERR_RUNTIME, "[%s] no kernel for tokens_per_page %d (supported: multiples of 8 up to %d)", op,
-                  tokens_per_page, kMaxPageSize);
-  } else if (tokens_per_page != 16 && tokens_per_page != 32) {
-    return fail(PAL_ERR_RUNTIME, "[%s] no kernel for tokens_per_page %d (supported: 16, 32)", op, tokens_per_page);
-  }
-  return PAL_OK;
 }
 
 size_t decode_workspace_size(int dtype, int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
@@ -595,142 +536,6 @@ int decode_call(const void* queries, const void* k_pool, const void* v_pool, con
                     "paged_attention_decode");
 }
 
-bool diff_head_dim_supported(int hd, bool kv8) { return hd == 64 || hd == 128 || (!kv8 && (hd == 32 || hd == 96)); }
-
-// The shapes of both differential attention entry points; returns PAL_OK or an error.
-int check_diff_dims(const char* op, int dtype, int kv_dtype, int num_q_heads, int num_kv_heads, int head_dim,
-                    int tokens_per_page, int64_t num_pages, int64_t page_table_width) {
-  const int st = check_attention_dims(op, dtype, num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages,
-                                      page_table_width);
-  if (st != PAL_OK) return st;
-  if (kv_dtype != dtype && kv_dtype != PAL_DTYPE_FP8_E4M3)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] pools must hold the queries' dtype or fp8 (dtype codes %d, %d)", op,
-                dtype, kv_dtype);
-  if (num_kv_heads % 2 != 0)
-    return fail(PAL_ERR_RUNTIME, "[%s] num_kv_heads must be even, two to a pair (%d)", op, num_kv_heads);
-  const bool kv8 = kv_dtype == PAL_DTYPE_FP8_E4M3;
-  if (!diff_head_dim_supported(head_dim, kv8))
-    return fail(PAL_ERR_RUNTIME, "[%s] no %skernel for head_dim %d (supported: %s)", op, kv8 ? "fp8 " : "", head_dim,
-                kv8 ? "64, 128" : "32, 64, 96, 128");
-  return PAL_OK;
-}
-
-// Workspace layout of a differential attention call (256-byte aligned offsets);
-// nothing in it needs initial contents.
-struct DiffLayout {
-  size_t cum, list, part_ml, part_o, total;
-};
-
-DiffLayout diff_layout(int64_t num_rows, int head_dim, int hg_max, int workers) {
-  const size_t rows = static_cast<size_t>(workers) * 2 * 2 * hg_max;  // partial rows
-  DiffLayout l;
-  l.cum = 256;  // behind the header
-  l.list = l.cum + align256(static_cast<size_t>(num_rows + 1) * sizeof(int64_t));
-  l.part_ml = l.list + align256(static_cast<size_t>(workers) * 4 * sizeof(int64_t));
-  l.part_o = l.part_ml + align256(rows * 2 * sizeof(float));
-  l.total = l.part_o + align256(rows * 2 * head_dim * sizeof(float));
-  return l;
-}
-
-int diff_heads_per_segment(int num_q_heads, int num_kv_heads) {
-  const int group = num_q_heads / num_kv_heads;
-  return group < 8 ? group : 8;
-}
-
-size_t diff_workspace_size(int dtype, int kv_dtype, int64_t num_rows, int num_q_heads, int num_kv_heads, int head_dim,
-                           int tokens_per_page) {
-  int workers = 0;
-  if (num_rows <= 0 || num_rows > 0x7fffffffLL ||
-      check_diff_dims("paged_differential_attention", dtype, kv_dtype, num_q_heads, num_kv_heads, head_dim,
-                      tokens_per_page, 0, 0) != PAL_OK ||
-      pal::diff_resident_workers(&workers) != hipSuccess)
-    return 0;
-  return diff_layout(num_rows, head_dim, diff_heads_per_segment(num_q_heads, num_kv_heads), workers).total;
-}
-
-// Rows of sequences: row i of sequence i (decode: no map), or of query_to_seq_map[i].
-int diff_call(const char* op, bool mapped, const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
-              const float* k_scales, const float* v_scales, const uint32_t* page_table,
-              const int32_t* sequence_lengths, const uint32_t* query_to_seq_map, const int32_t* query_token_offset,
-              const float* lambdas, const float* norm_weight, float norm_eps, float out_scale, void* out, int dtype,
-              int64_t num_rows, int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
-              int tokens_per_page, int64_t num_pages, int64_t page_table_width, void* workspace,
-              size_t workspace_bytes, hipStream_t stream) {
-  const int st = check_diff_dims(op, dtype, kv_dtype, num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages,
-                                 page_table_width);
-  if (st != PAL_OK) return st;
-  const bool kv8 = kv_dtype == PAL_DTYPE_FP8_E4M3;
-  if (kv8 != (k_scales != nullptr) || kv8 != (v_scales != nullptr))
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] k_scales and v_scales go with fp8 pools, both", op);
-  if (num_rows < 0 || num_seqs < 0) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] negative dimension", op);
-  if (num_rows > 0x7fffffffLL || num_seqs > 0x7fffffffLL || page_table_width > 0x7fffffffLL / tokens_per_page)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] problem too large for one call", op);
-  if (!(norm_eps >= 0.f)) return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] norm_eps must not be negative", op);
-  if (num_rows == 0) return ok();
-  if (num_pages == 0) page_table_width = 0;  // no page to read: every row is empty
-  if (!queries || !sequence_lengths || !lambdas || !out || (num_pages > 0 && (!k_pool || !v_pool)) ||
-      (page_table_width > 0 && !page_table) || (mapped && (!query_to_seq_map || !query_token_offset)))
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] null pointer argument", op);
-  if (!aligned16(queries) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(norm_weight) || !aligned16(out))
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] queries, pools, norm_weight and out must be 16-byte aligned", op);
-  int workers = 0;
-  const hipError_t err = pal::diff_resident_workers(&workers);
-  if (err != hipSuccess) return hip_status(err, op);
-  const int hg_max = diff_heads_per_segment(num_q_heads, num_kv_heads);
-  const DiffLayout lay = diff_layout(num_rows, head_dim, hg_max, workers);
-  if (workspace == nullptr || workspace_bytes < lay.total)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace of %zu bytes needed, %zu given", op, lay.total,
-                workspace_bytes);
-  if (reinterpret_cast<uintptr_t>(workspace) & 255u)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] workspace must be 256-byte aligned", op);
-  pal::DiffParams p{};
-  p.q = static_cast<const uint16_t*>(queries);
-  p.k_pool = k_pool;
-  p.v_pool = v_pool;
-  p.k_scales = k_scales;
-  p.v_scales = v_scales;
-  p.page_table = page_table;
-  p.seq_lens = sequence_lengths;
-  p.out = static_cast<uint16_t*>(out);
-  p.q2seq = mapped ? query_to_seq_map : nullptr;
-  p.q_offset = mapped ? query_token_offset : nullptr;
-  p.num_pt_rows = num_seqs;
-  p.num_seqs = num_rows;
-  p.num_pages = num_pages;
-  p.page_table_width = page_table_width;
-  p.num_q_heads = num_q_heads;
-  p.num_kv_heads = num_kv_heads / 2;
-  p.group = num_q_heads / num_kv_heads;
-  p.head_chunks = (p.group + 7) / 8;
-  p.hg_max = hg_max;
-  p.num_workers = workers;
-  p.tile_chunks = (p.group + 15) / 16;
-  p.tile_heads = (p.group + p.tile_chunks - 1) / p.tile_chunks;
-  p.tile_magic = (65536u + p.tile_heads - 1) / p.tile_heads;
-  const int64_t tile_rows = 128 / p.tile_heads;
-  const int64_t windows = (num_rows + tile_rows - 1) / tile_rows;
-  if (windows * p.num_kv_heads * p.tile_chunks > 0x7fffffffLL)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] problem too large for one call", op);
-  p.num_windows = static_cast<int>(windows);
-  p.scale_log2 = scale_log2_for(head_dim);
-  char* ws = static_cast<char*>(workspace);
-  p.hdr = reinterpret_cast<int64_t*>(ws);
-  p.claim = reinterpret_cast<uint32_t*>(ws + 128);
-  p.cum = reinterpret_cast<int64_t*>(ws + lay.cum);
-  p.split_list = reinterpret_cast<int64_t*>(ws + lay.list);
-  p.list_cap = workers;
-  p.part_ml = reinterpret_cast<float*>(ws + lay.part_ml);
-  p.part_o32 = reinterpret_cast<float*>(ws + lay.part_o);
-  p.lambdas = lambdas;
-  p.norm_weight = norm_weight;
-  p.norm_eps = norm_eps;
-  p.out_scale = out_scale;
-  PAL_LOG("%s rows=%lld seqs=%lld Hq=%d Hkv=%d HD=%d TPP=%d dtype=%d kv=%d norm=%d stream=%p", op,
-          static_cast<long long>(num_rows), static_cast<long long>(num_seqs), num_q_heads, num_kv_heads, head_dim,
-          tokens_per_page, dtype, kv_dtype, norm_weight ? 1 : 0, static_cast<void*>(stream));
-  return hip_status(pal::launch_diff(p, dtype, head_dim, tokens_per_page, stream), op);
-}
-
 }  // namespace
 
 extern "C" {
@@ -1011,45 +816,6 @@ int pal_paged_attention_fp8(const void* queries, const void* k_pool, const void*
                     query_token_offset, out, dtype, num_query_rows, num_seqs, num_q_heads, num_kv_heads, head_dim,
                     tokens_per_page, num_pages, page_table_width, workspace, workspace_bytes,
                     static_cast<hipStream_t>(stream));
-}
-
-size_t pal_paged_differential_attention_workspace_size(int dtype, int kv_dtype, int64_t num_query_rows,
-                                                       int num_q_heads, int num_kv_heads, int head_dim,
-                                                       int tokens_per_page) {
-  return diff_workspace_size(dtype, kv_dtype, num_query_rows, num_q_heads, num_kv_heads, head_dim, tokens_per_page);
-}
-
-int pal_paged_differential_attention_decode(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
-                                            const float* k_scales, const float* v_scales, const uint32_t* page_table,
-                                            const int32_t* sequence_lengths, const float* lambdas,
-                                            const float* norm_weight, float norm_eps, float out_scale, void* out,
-                                            int dtype, int64_t num_query_rows, int64_t num_seqs, int num_q_heads,
-                                            int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages,
-                                            int64_t page_table_width, void* workspace, size_t workspace_bytes,
-                                            void* stream) {
-  const char* op = "paged_differential_attention_decode";
-  if (num_query_rows < num_seqs)
-    return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] %lld query rows for %lld sequences", op,
-                static_cast<long long>(num_query_rows), static_cast<long long>(num_seqs));
-  return diff_call(op, false, queries, k_pool, v_pool, kv_dtype, k_scales, v_scales, page_table, sequence_lengths,
-                   nullptr, nullptr, lambdas, norm_weight, norm_eps, out_scale, out, dtype, num_seqs, num_seqs,
-                   num_q_heads, num_kv_heads, head_dim, tokens_per_page, num_pages, page_table_width, workspace,
-                   workspace_bytes, static_cast<hipStream_t>(stream));
-}
-
-int pal_paged_differential_attention(const void* queries, const void* k_pool, const void* v_pool, int kv_dtype,
-                                     const float* k_scales, const float* v_scales, const uint32_t* page_table,
-                                     const int32_t* sequence_lengths, const uint32_t* query_to_seq_map,
-                                     const int32_t* query_token_offset, const float* lambdas,
-                                     const float* norm_weight, float norm_eps, float out_scale, void* out, int dtype,
-                                     int64_t num_query_rows, int64_t num_seqs, int num_q_heads, int num_kv_heads,
-                                     int head_dim, int tokens_per_page, int64_t num_pages, int64_t page_table_width,
-                                     void* workspace, size_t workspace_bytes, void* stream) {
-  return diff_call("paged_differential_attention", true, queries, k_pool, v_pool, kv_dtype, k_scales, v_scales,
-                   page_table, sequence_lengths, query_to_seq_map, query_token_offset, lambdas, norm_weight, norm_eps,
-                   out_scale, out, dtype, num_query_rows, num_seqs, num_q_heads, num_kv_heads, head_dim,
-                   tokens_per_page, num_pages, page_table_width, workspace, workspace_bytes,
-                   static_cast<hipStream_t>(stream));
 }
 
 int pal_copy_pages(void* k_pool, void* v_pool, float* k_scales, float* v_scales, int64_t num_pages, int num_kv_heads,

@@ -182,11 +182,16 @@ struct DiffParams : DecodeParams {
   const float* norm_weight;  // [2 HD], or null: no norm
   float norm_eps;
   float out_scale;
+  // row mode: the rows alone in their run that have keys ({row, sequence, keys, 0}
+  // each, hdr[1] of them, for more than kInlinePlanSeqs rows), and the tiles ({first
+  // row, sequence}, hdr[2] of them, by falling work if hdr[3])
+  int32_t* lone;
+  uint32_t* tiles;
   // tiles of 128 M-rows: tile_heads output heads (at most 16) of tile_chunks groups
-  // per kv pair, num_windows windows of 128 / tile_heads rows
+  // per kv pair times up to tile_rows = 128 / tile_heads rows
   int tile_heads;
+  int tile_rows;
   int tile_chunks;
-  int num_windows;
   uint32_t tile_magic;       // ceil(2^16 / tile_heads): m / tile_heads = m * tile_magic >> 16 for m < 4096
   float* part_o32;           // [virtual workers][2][2 maps][hg_max][2 HD], not normalised (part_ml likewise: max, exp-sum)
 };

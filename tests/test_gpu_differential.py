@@ -260,6 +260,43 @@ def test_many_rows():
     run(chunk_case(16, lens, [(0, 700), (30, 600)], 4, 2, 32, 16, "bf16"), "1,500 lone rows and two chunks")
 
 
+@pytest.mark.parametrize("rows,longest", [(900, 4), (5000, 4), (9000, 2), (9000, 300)])
+def test_many_runs(rows, longest):
+    """Runs of 1 to `longest` rows with keys of any number: more tiles than the card holds at once, and than are put
+    in order (4,096), on either side of the 1,024 rows that are planned in the stream kernel."""
+    rng = np.random.default_rng(rows + longest)
+    seqs = 40
+    case = make_paged_case(rows, [0] + rng.integers(1, 400, seqs - 1).tolist(), 4, 4, 32, 16, "bf16")
+    q2s = []
+    while len(q2s) < rows:
+        s = int(rng.integers(0, seqs + 1))
+        if not q2s or s != q2s[-1]:
+            q2s += [s] * (2 if longest == 2 else int(rng.integers(1, longest + 1)))
+    q2s = np.array(q2s[:rows], np.uint32)
+    off = rng.integers(0, 450, rows).astype(np.int32)
+    q = randn_bits(rng, (rows, 4, 32), "bf16")
+    run(Diff(case, q, q2s, off, seed=rows), f"{rows} rows in runs of up to {longest}")
+
+
+def test_long_page_table():
+    """A page table of more steps than the order's buckets hold."""
+    case = make_paged_case(45, [70000, 40, 33000], 2, 2, 32, 16, "bf16")
+    q2s = np.repeat(np.array([0, 1, 2, 0, 2], np.uint32), [130, 20, 40, 1, 1])
+    off = np.concatenate([69000 + np.arange(130), 20 + np.arange(20), np.arange(40) * 800, [70000], [5]]).astype(np.int32)
+    q = randn_bits(np.random.default_rng(45), (len(q2s), 2, 32), "bf16")
+    run(Diff(case, q, q2s, off, seed=45), "a table of 70,000 keys")
+
+
+def test_no_sequences():
+    """Rows that all name no sequence, with a page table of no rows."""
+    d = chunk_case(46, [40], [(0, 10)], 4, 2, 64, 16, "bf16")
+    x = d.dev
+    n = torch.zeros(0, dtype=torch.int32, device=DEV)
+    out = pal.paged_differential_attention(x["q"], x["k"], x["v"], x["pt"][:0], n, x["q2s"], x["off"], x["lam"])
+    torch.cuda.synchronize()
+    assert tuple(out.shape) == (11, 2, 128) and not out.any()
+
+
 def test_any_limits_in_a_run():
     """Offsets of a run in any order, past the length, zero and negative; rows naming no sequence."""
     rng = np.random.default_rng(17)
