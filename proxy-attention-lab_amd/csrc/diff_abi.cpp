@@ -120,6 +120,13 @@ int diff_call(const char* op, bool mapped, const void* queries, const void* k_po
   p.tile_heads = (p.group + p.tile_chunks - 1) / p.tile_chunks;
   p.tile_magic = (65536u + p.tile_heads - 1) / p.tile_heads;
   p.tile_rows = 128 / p.tile_heads;
+  {  // 2^l / tile_rows rounded up, exact for x < 2^31 (tile_rows is 8 or more)
+    int log2 = 3;
+    while (2 << log2 <= p.tile_rows) ++log2;
+    const bool pow2 = 1 << log2 == p.tile_rows;
+    p.rows_shift = static_cast<uint32_t>(pow2 ? log2 - 1 : log2);
+    p.rows_magic = pow2 ? 1u << 31 : static_cast<uint32_t>((1ull << (32 + log2)) / p.tile_rows + 1);
+  }
   if ((num_rows / 2 + 1) * p.num_kv_heads * p.tile_chunks > 0x7fffffffLL)
     return fail(PAL_ERR_INVALID_ARGUMENT, "[%s] problem too large for one call", op);
   p.scale_log2 = scale_log2_for(head_dim);

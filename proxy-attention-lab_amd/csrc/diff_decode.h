@@ -49,130 +49,154 @@ struct DiffPlanLds {
 
 // The plan of a mixed batch's rows, by one workgroup of T threads: the lone rows
 // (alone in their run of rows of one sequence) with keys, and the tiles of the
-// longer runs, each run cut from its first row on.  Tiles are put in order of
-// falling work (the keys of their first row), so that the last ones to start are
-// short: 8 chunks of 512-2,048 rows on 0-2,048 cached, mean end of the workgroups
-// 412 us, last 483 us without.  (A counting sort; equal tiles fall in any order,
-// which changes no result.)  Lone rows without keys get their zeros.
-constexpr int kSortTiles = 4096;     // tiles put in order, at most (more: as they come)
-constexpr int kTileBuckets = 1024;   // of a step of 32 keys, or more for page tables past 32,768 keys
-constexpr int kPlanRows = 16;        // rows of a thread in a sweep
+// longer runs, each run cut from its first row on.  More tiles than the card
+// takes at once are put in order of falling work (the keys of their first row),
+// so that the last ones to start are short: 8 chunks of 512-2,048 rows on
+// 0-2,048 cached, mean end of the workgroups 412 us, last 483 us without.  (A
+// counting sort; equal tiles fall in any order, which changes no result.)  Lone
+// rows without keys get their zeros.
+//
+// One compute unit runs all of it, so its time is the instructions per row: the
+// rows are only searched for the starts of runs (ballots over groups of 64 rows,
+// loads a sweep ahead), and what follows works on the runs found.
+constexpr int kSortTiles = 4096;    // tiles put in order, at most (more: as they come)
+constexpr int kTileBuckets = 1024;  // of a step of 32 keys, or more for page tables past 32,768 keys
+constexpr int kPlanRows = 4;        // groups of a wavefront in a sweep
+constexpr int kPlanRuns = 6144;     // starts of runs kept: a sweep's (4,096), and of some before it
 template <int T>
 struct DiffRowsLds {
   uint32_t start[kTileBuckets];
   u32x2 tile[kSortTiles];
-  uint16_t key[kSortTiles];
-  int64_t sums[3][T / kWave];
-  int64_t totals[4];
+  union {
+    uint32_t run[kPlanRuns];
+    uint16_t key[kSortTiles];
+  };
+  int64_t sums[T / kWave];
+  int64_t total[2];
+  uint32_t found[T / kWave];
 };
 template <int T, int kPer, int HD, int TPP>
 __device__ __forceinline__ void diff_plan_rows(const DiffParams& p, DiffRowsLds<T>& L, bool keep_lone) {
+  constexpr int kWaves = T / kWave;
+  static_assert(T * kPer < kPlanRuns);
   const int tid = threadIdx.x;
-  const int64_t n = p.num_seqs;
+  const int lane = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t n = static_cast<uint32_t>(p.num_seqs);
   const int64_t max_tokens = p.page_table_width * TPP;
   const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
-  const int per_bucket = max(32, static_cast<int>((max_tokens + kTileBuckets - 1) / kTileBuckets));
-  auto keys_of = [&](uint32_t sq, int64_t r) {
+  auto keys_of = [&](uint32_t sq, uint32_t r) {
     if (sq >= p.num_pt_rows) return static_cast<int64_t>(0);
-    const int64_t k = min(p.seq_lens[sq], p.q_offset[r]);
+    const int64_t off = p.q_offset[r], all = p.seq_lens[sq];
+    const int64_t k = off < all ? off : all;
     PAL_DEBUG_FLAG(k > max_tokens, kDebugLength);
     return k < 0 ? static_cast<int64_t>(0) : (k > max_tokens ? max_tokens : k);
   };
-  for (int b = tid; b < kTileBuckets; b += T) L.start[b] = 0;
-  int64_t n_lone = 0, n_blocks = 0, n_tiles = 0, run = 0;  // so far; the first row of the run that a sweep starts in
-  for (int64_t base = 0; base < n; base += static_cast<int64_t>(T) * kPer) {
-    const int64_t r0 = base + static_cast<int64_t>(tid) * kPer;
-    uint32_t sq[kPer + 2];  // sequences of rows r0 - 1 .. r0 + kPer
-#pragma unroll
-    for (int k = 0; k < kPer + 2; ++k) {
-      const int64_t r = r0 - 1 + k;
-      sq[k] = r >= 0 && r < n ? p.q2seq[r] : 0u;
-    }
-    auto starts = [&](int k) { return r0 + k == 0 || sq[k] != sq[k + 1]; };          // row k starts a run
-    auto ends = [&](int k) { return r0 + k + 1 == n || sq[k + 2] != sq[k + 1]; };  // and ends one
-    // the run that row r0 lies in: the last start before it in the sweep, or the run it began in
-    int64_t last = -1;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k)
-      if (r0 + k < n && starts(k)) last = r0 + k;
-    int64_t before = last;  // running maximum over the threads, then of those before this one
-    {
-      const int lane = lane_id();
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const int64_t o = __shfl_up(before, off, kWave);
-        if (lane >= off) before = max(before, o);
-      }
-      if (lane == kWave - 1) L.sums[0][tid >> 6] = before;
-      before = __shfl_up(before, 1, kWave);
-      if (lane == 0) before = -1;
-      __syncthreads();
-      for (int i = 0; i < (tid >> 6); ++i) before = max(before, L.sums[0][i]);
-      if (before < 0) before = run;
-      if (tid == T - 1) L.totals[3] = last >= 0 ? last : before;
-      __syncthreads();
-    }
-    // this thread's lone rows and tile starts
-    int64_t lone = 0, blocks = 0, tiles = 0, at = before;
-    uint32_t is_tile = 0;
-    int32_t len[kPer];
+  const uint64_t lower = (1ull << lane) - 1;  // the lanes before this one
+  // rows of a wavefront: as few groups as hold the batch
+  const uint32_t need = (n + T - 1) / T;
+  const uint32_t groups = need < kPer ? need : kPer;
+  uint32_t n_lone = 0, n_tiles = 0, n_runs = 0;  // so far; runs in L.run
+  int64_t n_blocks = 0;
+  uint32_t sq[kPer], edge;  // loaded a sweep ahead: the wavefront's rows, the row before them
+  auto load = [&](uint32_t w0) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      len[k] = 0;
-      if (r0 + k >= n) continue;
-      if (starts(k)) at = r0 + k;
-      if (at == r0 + k && ends(k)) {
-        len[k] = static_cast<int32_t>(keys_of(sq[k + 1], r0 + k));
-        if (len[k] > 0) {
-          lone += 1;
-          blocks += ((len[k] + 15) >> 4) * segs;
-        } else if (keep_lone) {
-          zero_item_output<HD>(p, r0 + k);
-        }
-      } else if (static_cast<uint32_t>(r0 + k - at) % static_cast<uint32_t>(p.tile_rows) == 0) {
-        tiles += 1;
-        is_tile |= 1u << k;
-      }
+      const uint32_t r = w0 + k * kWave + lane;
+      sq[k] = static_cast<uint32_t>(k) < groups && r < n ? p.q2seq[r] : 0u;
     }
-    const int64_t lone_to = block_inclusive_scan<T>(lone, L.sums[0]);
-    const int64_t blocks_to = block_inclusive_scan<T>(blocks, L.sums[1]);
-    const int64_t tiles_to = block_inclusive_scan<T>(tiles, L.sums[2]);
-    int64_t li = n_lone + lone_to - lone, bi = n_blocks + blocks_to - blocks, ti = n_tiles + tiles_to - tiles;
+    edge = w0 > 0 && w0 <= n ? p.q2seq[w0 - 1] : 0u;
+  };
+  load(static_cast<uint32_t>(w) * kWave * groups);
+#pragma unroll 1
+  for (uint32_t base = 0; base < n; base += T * groups) {
+    const uint32_t w0 = base + static_cast<uint32_t>(w) * kWave * groups;
+    uint64_t starts[kPer];
+    uint32_t prev = edge, mine = 0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      if (len[k] > 0 && keep_lone) {
-        *reinterpret_cast<u32x4*>(p.lone + 4 * li) =
-            u32x4{static_cast<uint32_t>(r0 + k), sq[k + 1], static_cast<uint32_t>(len[k]), 0u};
-        p.cum[li] = bi;
-        li += 1;
-        bi += ((len[k] + 15) >> 4) * segs;
-      }
-      if (is_tile >> k & 1) {
-        const u32x2 t = {static_cast<uint32_t>(r0 + k), sq[k + 1]};
-        if (ti < kSortTiles) {
-          const int64_t b = keys_of(sq[k + 1], r0 + k) / per_bucket;
-          const int key = kTileBuckets - 1 - static_cast<int>(b < kTileBuckets - 1 ? b : kTileBuckets - 1);
-          L.tile[ti] = t;
-          L.key[ti] = static_cast<uint16_t>(key);
-          atomicAdd(&L.start[key], 1u);
-        } else {
-          *reinterpret_cast<u32x2*>(p.tiles + 2 * ti) = t;
-        }
-        ti += 1;
-      }
+      const uint32_t r = w0 + k * kWave + lane;
+      uint32_t left = __shfl_up(sq[k], 1, kWave);
+      if (lane == 0) left = prev;
+      prev = __builtin_amdgcn_readlane(sq[k], kWave - 1);
+      starts[k] = __ballot(static_cast<uint32_t>(k) < groups && r < n && (r == 0 || left != sq[k]));
+      mine += __builtin_popcountll(starts[k]);
     }
-    if (tid == T - 1) {
-      L.totals[0] = lone_to;
-      L.totals[1] = blocks_to;
-      L.totals[2] = tiles_to;
+    load(w0 + T * groups);
+    if (lane == 0) L.found[w] = mine;
+    __syncthreads();
+    uint32_t at = n_runs;
+    for (int i = 0; i < kWaves; ++i) {
+      const uint32_t f = L.found[i];
+      at += i < w ? f : 0u;
+      n_runs += f;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (starts[k] >> lane & 1) L.run[at + __builtin_popcountll(starts[k] & lower)] = w0 + k * kWave + lane;
+      at += __builtin_popcountll(starts[k]);
     }
     __syncthreads();
-    n_lone += L.totals[0];
-    n_blocks += L.totals[1];
-    n_tiles += L.totals[2];
-    run = L.totals[3];
-    __syncthreads();
+    const bool end = base + T * groups >= n;
+    if (!end && n_runs + T * groups <= kPlanRuns) continue;
+    // The runs with a known end: all at the end of the rows, else all but the last.
+    const uint32_t done = end ? n_runs : n_runs - 1;
+#pragma unroll 1
+    for (uint32_t j = 0; j < done; j += T) {
+      const uint32_t i = j + tid;
+      const bool in = i < done;
+      const uint32_t row = in ? L.run[i] : 0u;
+      const uint32_t rows = in ? (i + 1 < n_runs ? L.run[i + 1] : n) - row : 0u;
+      const uint32_t seq = in ? p.q2seq[row] : 0u;
+      int64_t keys = 0;
+      if (rows == 1 && keep_lone) {
+        keys = keys_of(seq, row);
+        if (keys == 0) zero_item_output<HD>(p, row);
+      }
+      const uint32_t tiles = rows > 1 ? (__umulhi(rows - 1, p.rows_magic) >> p.rows_shift) + 1 : 0u;
+      const int64_t count = static_cast<int64_t>(keys > 0) << 32 | tiles;
+      const int64_t count_to = block_inclusive_scan<T>(count, L.sums);
+      const int64_t blocks = ((keys + 15) >> 4) * segs;
+      const int64_t blocks_to = keep_lone ? block_inclusive_scan<T>(blocks, L.sums) : 0;
+      if (tid == T - 1) {
+        L.total[0] = count_to;
+        L.total[1] = blocks_to;
+      }
+      if (keys > 0) {
+        const int64_t li = n_lone + static_cast<uint32_t>((count_to - count) >> 32);
+        *reinterpret_cast<u32x4*>(p.lone + 4 * li) = u32x4{row, seq, static_cast<uint32_t>(keys), 0u};
+        p.cum[li] = n_blocks + blocks_to - blocks;
+      }
+      auto put = [&](uint32_t i, uint32_t row, uint32_t seq) {
+        const u32x2 t = {row, seq};
+        if (i < kSortTiles)
+          L.tile[i] = t;
+        else
+          *reinterpret_cast<u32x2*>(p.tiles + 2 * static_cast<int64_t>(i)) = t;
+      };
+      const uint32_t ti = n_tiles + static_cast<uint32_t>(count_to - count);
+      if (tiles == 1) put(ti, row, seq);
+      for (uint64_t more = __ballot(tiles > 1); more; more &= more - 1) {  // longer runs: by the wavefront
+        const int l = __builtin_ctzll(more);
+        const uint32_t c = __builtin_amdgcn_readlane(tiles, l), t0 = __builtin_amdgcn_readlane(ti, l);
+        const uint32_t r0 = __builtin_amdgcn_readlane(row, l), sq0 = __builtin_amdgcn_readlane(seq, l);
+        for (uint32_t m = lane; m < c; m += kWave) put(t0 + m, r0 + m * p.tile_rows, sq0);
+      }
+      __syncthreads();
+      n_lone += static_cast<uint32_t>(L.total[0] >> 32);
+      n_tiles += static_cast<uint32_t>(L.total[0]);
+      n_blocks += L.total[1];
+      __syncthreads();
+    }
+    if (!end) {
+      const uint32_t open = L.run[done];
+      __syncthreads();
+      if (tid == 0) L.run[0] = open;
+      n_runs = 1;
+    }
   }
+  const int64_t items = static_cast<int64_t>(n_tiles) * p.num_kv_heads * p.tile_chunks;
+  const bool sort = items > p.num_workers / kDiffWaves && n_tiles <= kSortTiles;
   if (tid == 0) {
     if (keep_lone) {
       p.hdr[0] = n_blocks;
@@ -180,17 +204,30 @@ __device__ __forceinline__ void diff_plan_rows(const DiffParams& p, DiffRowsLds<
       p.cum[n_lone] = n_blocks;
     }
     p.hdr[2] = n_tiles;
-    p.hdr[3] = n_tiles <= kSortTiles;
+    p.hdr[3] = sort;
   }
-  if (n_tiles > kSortTiles) {  // too many: in the rows' order
-    for (int i = tid; i < kSortTiles; i += T) *reinterpret_cast<u32x2*>(p.tiles + 2 * i) = L.tile[i];
+  if (sort)
+    for (int b = tid; b < kTileBuckets; b += T) L.start[b] = 0;
+  __syncthreads();
+  if (!sort) {  // in the rows' order
+    for (uint32_t i = tid; i < n_tiles && i < kSortTiles; i += T)
+      *reinterpret_cast<u32x2*>(p.tiles + 2 * i) = L.tile[i];
     return;
   }
+  const int per_bucket = max(32, static_cast<int>((max_tokens + kTileBuckets - 1) / kTileBuckets));
+  for (uint32_t i = tid; i < n_tiles; i += T) {
+    const u32x2 t = L.tile[i];
+    const uint32_t b = static_cast<uint32_t>(keys_of(t.y, t.x)) / static_cast<uint32_t>(per_bucket);
+    const uint32_t key = kTileBuckets - 1 - (b < kTileBuckets - 1 ? b : kTileBuckets - 1);
+    L.key[i] = static_cast<uint16_t>(key);
+    atomicAdd(&L.start[key], 1u);
+  }
+  __syncthreads();
   constexpr int kB = kTileBuckets / T;
   int64_t sum = 0;
 #pragma unroll
   for (int k = 0; k < kB; ++k) sum += L.start[tid * kB + k];
-  int64_t at = block_inclusive_scan<T>(sum, L.sums[0]) - sum;
+  int64_t at = block_inclusive_scan<T>(sum, L.sums) - sum;
 #pragma unroll
   for (int k = 0; k < kB; ++k) {
     const uint32_t c = L.start[tid * kB + k];
@@ -198,7 +235,7 @@ __device__ __forceinline__ void diff_plan_rows(const DiffParams& p, DiffRowsLds<
     at += c;
   }
   __syncthreads();
-  for (int64_t i = tid; i < n_tiles; i += T)
+  for (uint32_t i = tid; i < n_tiles; i += T)
     *reinterpret_cast<u32x2*>(p.tiles + 2 * atomicAdd(&L.start[L.key[i]], 1u)) = L.tile[i];
 }
 

@@ -191,6 +191,7 @@ struct DiffParams : DecodeParams {
   // per kv pair times up to tile_rows = 128 / tile_heads rows
   int tile_heads;
   int tile_rows;
+  uint32_t rows_magic, rows_shift;  // x / tile_rows = umulhi(x, magic) >> shift for x < 2^31
   int tile_chunks;
   uint32_t tile_magic;       // ceil(2^16 / tile_heads): m / tile_heads = m * tile_magic >> 16 for m < 4096
   float* part_o32;           // [virtual workers][2][2 maps][hg_max][2 HD], not normalised (part_ml likewise: max, exp-sum)
