@@ -256,9 +256,20 @@ __device__ __forceinline__ float lane_xor8(float x) {
 // piece boundaries: while the last blocks of a piece are computed, the first
 // of the next piece are loading (its item, query and first page ids were fetched
 // when the piece before it started).
+// Descriptor of `bytes` bytes at a wavefront's common address: loads past them
+// read nothing and give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_descriptor(const uint8_t* at, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(at);
+  // (the builtin returns an int: without the casts a low half past 2^31 would be sign-extended)
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a)));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32)));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(hi) << 32 | lo), 0, bytes,
+                                           0x00027000);
+}
+
 template <int DT, int HD, int TPP, int PF, bool KV8>
 __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc, const int64_t* cum,
-                                           const DiffPlanLds* plan, int64_t n_items, int64_t v) {
+                                           const DiffPlanLds* plan, int64_t n_items, const float* weight, int64_t v) {
   static_assert(HD % 32 == 0 && (!KV8 || HD % 64 == 0), "whole k-steps and stripes");
   constexpr int KK = HD / 32;     // QK k-steps of 32 dims of one map
   constexpr int NT = 2 * HD / 16;  // output tiles of 16 dims
@@ -340,13 +351,17 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
 
   // Q^T operand of a piece: the dims of this lane's k-slices of its column's
   // query (zeros in columns without a head).
+  // Its lambda comes with it: a load at the piece's end would wait for the next
+  // piece's blocks, in flight by then.
   u32x4 qv[KK], qn[KK];
-  auto load_q = [&](int64_t row, int seg, u32x4 (&q)[KK]) {
+  float lam, lam_n;
+  auto load_q = [&](int64_t row, int seg, u32x4 (&q)[KK], float& l) {
     const int h0 = (seg % p.head_chunks) * 8;
     const bool hv = r8 < min(8, p.group - h0);
     const uint32_t qmask = hv ? 0xFFFFFFFFu : 0u;
     const int64_t head = static_cast<int64_t>(seg / p.head_chunks) * p.group + h0 + (hv ? r8 : 0);
     const uint16_t* qrow = p.q + (row * p.num_q_heads + 2 * head + map) * HD;
+    l = p.lambdas[head];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       if constexpr (KV8)  // k-step kk = (stripe g + 4 (kk / 2), half kk % 2)
@@ -366,7 +381,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     const int64_t s0 = locate_seq(cum, n_items, b0);  // the item holding block b0 (it has blocks)
     PAL_FIND_PIECE(c_, s0, b0 - cum[s0], b0);
   }
-  load_q(c_row, c_seg, qv);
+  load_q(c_row, c_seg, qv, lam);
 
   // Page ids in register windows of 64 pages: pid_cur holds window wcur, the
   // window of the block being computed, pid_nxt the next one; every step group
@@ -409,23 +424,17 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     int bstart_n = 0, pbase_n = 0;
 
     // Issues the loads of step i of the piece into buffer `buf`: block i of the
-    // piece (clamped to its last) or, past the piece's steps, block i - n_pad of
-    // the next piece.  An out-of-range page id reads page 0 and the block is
-    // masked when computed.  Every block is read once per call: non-temporal,
-    // but for 32-token pages, whose rows this block and the next share (as in
-    // ordinary decode: cacheable where a kv head's block holds 8 KiB or more).
-    constexpr bool kCached = TPP == 32 && 2 * HD * TPP * EB >= 8192;
-    auto load16 = [](const uint8_t* a) {
-      if constexpr (kCached) return *reinterpret_cast<const u32x4*>(a);
-      else return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a));
-    };
-    auto load8 = [](const uint8_t* a) {
-      if constexpr (kCached) return *reinterpret_cast<const u32x2*>(a);
-      else return __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(a));
-    };
+    // piece or, past the piece's steps, block i - n_pad of the next piece.  They go
+    // through descriptors of the pair's block: a step past the piece's end, or with
+    // a page id out of range, takes one of no bytes, whose loads read no memory and
+    // give zeros (the block is masked when computed).  Every block is read once per
+    // call: non-temporal, but for 32-token pages, whose rows this block and the
+    // next share (as in ordinary decode: cacheable where a kv head's block holds
+    // 8 KiB or more).
+    constexpr int kPolicy = TPP == 32 && 2 * HD * TPP * EB >= 8192 ? 0 : 2;  // 2: non-temporal
     auto issue = [&](int i, int buf, uint32_t w_n0) {
       const bool to_next = has_next && i >= n_pad;
-      const int j = to_next ? (i - n_pad < nblk_n - 1 ? i - n_pad : nblk_n - 1) : (i < n_blk - 1 ? i : n_blk - 1);
+      const int j = to_next ? i - n_pad : i;
       const int b = (to_next ? bstart_n : bstart) + j;
       const int e = (b * 16) / TPP - (to_next ? pbase_n : pbase);  // page within the piece's windows
       // (selects of values: a select of two variables' addresses would push the
@@ -434,30 +443,41 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       const uint32_t win = to_next ? w_n0 : ((e >> 6) == wcur ? w_c : w_x);
       const uint32_t pg = __builtin_amdgcn_readlane(win, static_cast<int>(e & 63));
       bv[buf] = pg < p.num_pages;
-      PAL_DEBUG_FLAG(!bv[buf] && (to_next ? i - n_pad < nblk_n : i < n_blk), kDebugPageId);
-      const uint32_t page = bv[buf] ? pg : 0u;
-      const int slot0 = static_cast<int>((b * 16) % TPP);
+      const bool in = j < (to_next ? nblk_n : n_blk);
+      PAL_DEBUG_FLAG(!bv[buf] && in, kDebugPageId);
+      const bool ok = __builtin_amdgcn_readfirstlane(bv[buf] && in);
+      const uint32_t page = ok ? pg : 0u;
+      const uint32_t slot0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((b * 16) % TPP));
       const uint8_t* kb_x = kbase_n;
       const uint8_t* vb_x = vbase_n;
-      const uint8_t* kp = (to_next ? kb_x : kbase) + static_cast<int64_t>(page) * page_stride + (slot0 + r16) * 16;
-      const uint8_t* vp = (to_next ? vb_x : vbase) + static_cast<int64_t>(page) * page_stride + slot0 * EB;
+      const int bytes = ok ? static_cast<int>(2 * head_block) : 0;
+      const auto kd = block_descriptor((to_next ? kb_x : kbase) + static_cast<int64_t>(page) * page_stride, bytes);
+      const auto vd = block_descriptor((to_next ? vb_x : vbase) + static_cast<int64_t>(page) * page_stride, bytes);
       if constexpr (KV8) {
         const int64_t si = 2 * (static_cast<int64_t>(page) * p.num_kv_heads + (to_next ? pair_n : pair));
         bks[buf] = f32x2{p.k_scales[si], p.k_scales[si + 1]};
         bvs[buf] = f32x2{p.v_scales[si], p.v_scales[si + 1]};
       }
+      // (the empty asm keeps the sums with constants here, where they become the loads' offsets)
+      uint32_t k_at = (r16 + g * TPP) * 16;
+      uint32_t v_at = KV8 ? (16 * g + r16) * TPP : (r16 * TPP + 4 * g) * 2;
+      asm volatile("" : "+v"(k_at), "+v"(v_at));
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int kk = 0; kk < KL; ++kk) kb[buf][a][kk] = load16(kp + a * head_block + (4 * kk + g) * TPP * 16);
+        for (int kk = 0; kk < KL; ++kk)
+          kb[buf][a][kk] = __builtin_amdgcn_raw_buffer_load_b128(
+              kd, k_at + a * (HD * TPP * EB) + 4 * kk * TPP * 16, slot0 * 16, kPolicy);
       if constexpr (KV8) {
         // lane 16g + i reads the block's 16 codes of dim row 64q + 16g + i; compute
         // transposes them across the lane groups
 #pragma unroll
-        for (int q = 0; q < NT / 4; ++q) vq8[buf][q] = load16(vp + (64 * q + 16 * g + r16) * TPP);
+        for (int q = 0; q < NT / 4; ++q)
+          vq8[buf][q] = __builtin_amdgcn_raw_buffer_load_b128(vd, v_at + 64 * q * TPP, slot0, kPolicy);
       } else {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) vb[buf][n] = load8(vp + ((16 * n + r16) * TPP + 4 * g) * 2);
+        for (int n = 0; n < NT; ++n)
+          vb[buf][n] = __builtin_amdgcn_raw_buffer_load_b64(vd, v_at + 32 * n * TPP, slot0 * 2, kPolicy);
       }
     };
 
@@ -575,7 +595,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
         x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_row = c_row; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
         x_count = c_count; x_seg = c_seg;
       }
-      load_q(x_row, x_seg, qn);
+      load_q(x_row, x_seg, qn, lam_n);
       pidn0 = load_window(x_seq, x_blk, 0);
     }
     const uint32_t pidn1 = load_window(x_seq, x_blk, 1);
@@ -611,6 +631,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(qn[kk]));
       asm volatile("" ::"v"(pidn1));
+      asm volatile("" ::"v"(lam_n));
       asm volatile("v_mov_b32 %0, %1" : "=v"(pidn0_ready) : "v"(pidn0));
     };
     if (n_pad == NBUF) {
@@ -630,7 +651,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       // lane ^ 8, so both hold x; the norm sums it over the 4 lane groups
       const int64_t head = static_cast<int64_t>(pair) * p.group + h0 + (r8 < hg ? r8 : 0);
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // (no score above -inf: the map adds nothing)
-      const float f = map ? -p.lambdas[head] * inv : inv;
+      const float f = map ? -lam * inv : inv;
       float ss = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -641,8 +662,8 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
           ss += o[n][e] * o[n][e];
         }
       }
-      float scale = p.out_scale;
-      if (p.norm_weight) scale *= 1.f / sqrtf(sum_xor32(sum_xor16(ss)) * (1.f / (2 * HD)) + p.norm_eps);
+      float scale = 1.f;
+      if (p.norm_weight) scale = 1.f / sqrtf(sum_xor32(sum_xor16(ss)) * (1.f / (2 * HD)) + p.norm_eps);
       if (r8 < hg) {
         // the two lanes of a head write half of its row each
         uint16_t* row = p.out + (c_row * (p.num_q_heads / 2) + head) * (2 * HD) + 4 * g;
@@ -650,8 +671,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
         for (int n = 0; n < NT / 2; ++n) {
           const int t = n + map * (NT / 2);
           f32x4 y = map ? o[n + NT / 2] : o[n];
-          y *= scale;
-          if (p.norm_weight) y *= *reinterpret_cast<const f32x4*>(p.norm_weight + 16 * t + 4 * g);
+          y *= scale * *reinterpret_cast<const f32x4*>(weight + 16 * t + 4 * g);
           *reinterpret_cast<u32x2*>(row + 16 * t) = u32x2{Dt<DT>::pack2(y[0], y[1]), Dt<DT>::pack2(y[2], y[3])};
         }
       }
@@ -679,6 +699,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     c_count = x_count; c_seg = x_seg;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qv[kk] = qn[kk];
+    lam = lam_n;
     wcur = 0;
     pid_cur = pidn0;
     pid_nxt = pidn1;
@@ -695,6 +716,8 @@ void diff_stream_kernel(const DiffParams p) {
     DiffPlanLds plan;
     DiffRowsLds<kDiffThreads> rows;
   } lds_all;
+  // what a row is scaled with behind its norm (in LDS: see load_q)
+  __shared__ __attribute__((aligned(16))) float weight[2 * HD];
   DiffPlanLds& lds = lds_all.plan;
   const int64_t n = p.num_seqs;
   const int tid = threadIdx.x;
@@ -705,25 +728,57 @@ void diff_stream_kernel(const DiffParams p) {
     return;
   }
   if (blockIdx.x == 0 && tid < kDiffQueues) p.claim[tid] = 0;  // for the tiles, the launch behind
+  if (tid < 2 * HD) weight[tid] = p.out_scale * (p.norm_weight ? p.norm_weight[tid] : 1.f);
   int64_t n_items = n, total;
   const int64_t* cum = p.cum;
   const DiffPlanLds* plan = nullptr;
   if (scan) {
-    // every workgroup scans the lengths into LDS: thread t owns items 4t .. 4t+3
+    // every workgroup scans the lengths into LDS: thread t owns items 4t .. 4t+3,
+    // whose loads are in flight together
     const int64_t segs = static_cast<int64_t>(p.num_kv_heads) * p.head_chunks;
+    const int64_t max_tokens = p.page_table_width * TPP;
+    const int first = tid * kPer;
+    const int last = static_cast<int>(n) - 1;
+    uint32_t seq[kPer];
+    int64_t keys[kPer];
+    bool skip[kPer] = {};
+    if (p.q2seq) {
+      uint32_t sq[kPer + 2];
+      int32_t off[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer + 2; ++k) sq[k] = p.q2seq[max(0, min(first + k - 1, last))];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) off[k] = p.q_offset[min(first + k, last)];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int s = first + k;
+        skip[k] = (s > 0 && sq[k] == sq[k + 1]) || (s < last && sq[k + 2] == sq[k + 1]);  // a tile's row
+        const bool has = sq[k + 1] < p.num_pt_rows && !skip[k];
+        seq[k] = has ? sq[k + 1] : 0u;
+        const int32_t all = p.num_pt_rows ? p.seq_lens[seq[k]] : 0;
+        keys[k] = has ? min(all, off[k]) : 0;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        seq[k] = static_cast<uint32_t>(first + k);
+        keys[k] = p.seq_lens[min(first + k, last)];
+      }
+    }
     int64_t vals[kPer];
     int64_t tsum = 0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int64_t s = static_cast<int64_t>(tid) * kPer + k;
-      vals[k] = 0;
-      if (s < n) {
-        const Item it = item_at(p, s, TPP);
-        vals[k] = ((it.len + 15) >> 4) * segs;
-        lds.len[s] = static_cast<int32_t>(it.len);
-        lds.seq[s] = static_cast<int32_t>(it.seq);
-        lds.row[s] = static_cast<int32_t>(s);
-        if (it.len == 0 && !it.skip && blockIdx.x == 0) zero_item_output<HD>(p, it.row);
+      const int s = first + k;
+      const bool in = s <= last;
+      PAL_DEBUG_FLAG(in && keys[k] > max_tokens, kDebugLength);
+      const int64_t len = !in || keys[k] < 0 ? 0 : (keys[k] > max_tokens ? max_tokens : keys[k]);
+      vals[k] = ((len + 15) >> 4) * segs;
+      if (in) {
+        lds.len[s] = static_cast<int32_t>(len);
+        lds.seq[s] = static_cast<int32_t>(seq[k]);
+        lds.row[s] = s;
+        if (len == 0 && !skip[k] && blockIdx.x == 0) zero_item_output<HD>(p, s);
       }
       tsum += vals[k];
     }
@@ -758,10 +813,11 @@ void diff_stream_kernel(const DiffParams p) {
     }
   }
   if (plan) cum = plan->cum;
+  __syncthreads();
   if (total == 0) return;
   const Sched sc = make_sched(total, p.num_workers, 0);
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kDiffWaves + wave_id();
-  if (w < sc.nws) diff_range<DT, HD, TPP, KV8 ? 3 : 2, KV8>(p, sc, cum, plan, n_items, w);
+  if (w < sc.nws) diff_range<DT, HD, TPP, KV8 ? 3 : 2, KV8>(p, sc, cum, plan, n_items, weight, w);
 }
 
 // Joins the pieces of split segments: workgroup (v, h) takes head h of the
