@@ -118,7 +118,7 @@ __device__ __forceinline__ int64_t locate_seq(const int64_t* cum, int64_t num_se
 // it also writes the zeros of an empty item.
 constexpr int kPlanPer = 16;
 
-template <int HD, int TPP>
+template <int HD, int TPP, int kSegmentCost = 0>
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const DecodeParams p) {
   __shared__ int64_t wave_sums[kPlanThreads / kWave];
   __shared__ int64_t carry_sh;
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(const DecodeP
       vals[k] = 0;
       if (s < n) {
         const Item it = item_at(p, s, TPP);
-        vals[k] = ((it.len + 15) >> 4) * segs;
+        vals[k] = it.len > 0 ? (((it.len + 15) >> 4) + kSegmentCost) * segs : 0;
         if (it.len == 0 && !it.skip) zero_item_output<HD>(p, it.row);
       }
       tsum += vals[k];

@@ -36,6 +36,12 @@ namespace {
 constexpr int kDiffWaves = 4;  // independent wavefront workers per workgroup
 constexpr int kDiffThreads = kDiffWaves * kWave;
 constexpr int kDiffQueues = 8;       // claim counters of the tiles
+// What a segment costs a worker beyond its blocks, in blocks: the last group of
+// steps filled up, the segment's end.  Shares are cut from the blocks with so many
+// empty ones behind each segment; cut from the blocks alone, a worker of short
+// segments had twice the steps of the mean (1,000 x 1-256 keys, 16 kv heads:
+// 261 us, now 197).
+constexpr int kDiffSegmentCost = 3;
 constexpr float kDiffLazyMax = 8.f;  // log2 headroom before a running max moves
 
 // Up to kInlinePlanSeqs items of a batch, in LDS.
@@ -156,7 +162,7 @@ __device__ __forceinline__ void diff_plan_rows(const DiffParams& p, DiffRowsLds<
       const uint32_t tiles = rows > 1 ? (__umulhi(rows - 1, p.rows_magic) >> p.rows_shift) + 1 : 0u;
       const int64_t count = static_cast<int64_t>(keys > 0) << 32 | tiles;
       const int64_t count_to = block_inclusive_scan<T>(count, L.sums);
-      const int64_t blocks = ((keys + 15) >> 4) * segs;
+      const int64_t blocks = keys > 0 ? (((keys + 15) >> 4) + kDiffSegmentCost) * segs : 0;
       const int64_t blocks_to = keep_lone ? block_inclusive_scan<T>(blocks, L.sums) : 0;
       if (tid == T - 1) {
         L.total[0] = count_to;
@@ -309,7 +315,8 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
 
   // A piece: item s (row `row` of page-table row `seq`, `len` keys, nb blocks per segment),
   // segment `seg`, blocks [blk, blk + count) of the segment, from global block
-  // gpos on; r = block offset of the piece inside the item's segments.  c_* is
+  // gpos on; r = its place in the units of the item (a segment has nb +
+  // kDiffSegmentCost of them, as the global list has).  c_* is
   // the piece being computed, x_* the next one (kept in scalars).
   int64_t c_s, c_r, c_gpos, c_row, c_seq, c_len, c_nb, c_blk, c_count;
   int c_seg;
@@ -317,7 +324,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   int x_seg;
 #define PAL_FIND_PIECE(P, S0, R0, G0)                                                      \
   do {                                                                                     \
-    int64_t s_ = (S0), r_ = (R0), len_, seq_, row_;                                        \
+    int64_t s_ = (S0), r_ = (R0), g_ = (G0), len_, seq_, row_, nb_, unit_, seg_ = 0, blk_ = 0; \
     for (;;) {                                                                             \
       if (plan) {                                                                          \
         len_ = plan->len[s_];                                                              \
@@ -333,19 +340,29 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
         seq_ = it_.seq;                                                                    \
         row_ = s_;                                                                         \
       }                                                                                    \
-      if (len_ > 0) break;                                                                 \
+      nb_ = (len_ + 15) >> 4;                                                              \
+      unit_ = nb_ + kDiffSegmentCost;                                                      \
+      if (len_ > 0) {                                                                      \
+        seg_ = r_ / unit_;                                                                 \
+        blk_ = r_ - seg_ * unit_;                                                          \
+        if (blk_ < nb_) break;                                                             \
+        r_ += unit_ - blk_; /* behind a segment: on to the next */                         \
+        g_ += unit_ - blk_;                                                                \
+        if (g_ >= b_end) break;                                                            \
+        if (r_ < unit_ * segs) continue;                                                   \
+      }                                                                                    \
       ++s_;                                                                                \
       r_ = 0;                                                                              \
     }                                                                                      \
     P##s = s_;                                                                             \
     P##r = r_;                                                                             \
-    P##gpos = (G0);                                                                        \
+    P##gpos = g_;                                                                          \
     P##row = row_;                                                                         \
     P##seq = seq_;                                                                         \
     P##len = len_;                                                                         \
-    P##nb = (len_ + 15) >> 4;                                                              \
-    P##seg = static_cast<int>(r_ / P##nb);                                                 \
-    P##blk = r_ - P##seg * P##nb;                                                          \
+    P##nb = nb_;                                                                           \
+    P##seg = static_cast<int>(seg_);                                                       \
+    P##blk = blk_;                                                                         \
     P##count = (P##nb - P##blk) < (b_end - P##gpos) ? (P##nb - P##blk) : (b_end - P##gpos); \
   } while (0)
 
@@ -381,6 +398,10 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     const int64_t s0 = locate_seq(cum, n_items, b0);  // the item holding block b0 (it has blocks)
     PAL_FIND_PIECE(c_, s0, b0 - cum[s0], b0);
   }
+  if (c_gpos >= b_end) {  // the range lies behind a segment
+    write_list();
+    return;
+  }
   load_q(c_row, c_seg, qv, lam);
 
   // Page ids in register windows of 64 pages: pid_cur holds window wcur, the
@@ -397,7 +418,6 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
   f32x2 bks[NBUF], bvs[NBUF];  // fp8: the block's scales, of kv heads 2j and 2j + 1
   bool bv[NBUF];
 
-  bool first = true;     // the piece is the worker's first
   bool prologue = true;  // the pipeline is empty
   bool has_next = false;
   x_s = c_s; x_r = c_r; x_gpos = c_gpos; x_row = c_row; x_seq = c_seq; x_len = c_len; x_nb = c_nb; x_blk = c_blk;
@@ -582,10 +602,11 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
     // The next piece: its item, query and first page ids load now, while this
     // piece streams (with none, the current one's again: no load under a branch).
     {
-      const int64_t gpos_n = c_gpos + c_count;
+      const int64_t past = c_count + (c_blk + c_count == c_nb ? kDiffSegmentCost : 0);
+      const int64_t gpos_n = c_gpos + past;
       has_next = gpos_n < b_end;
-      int64_t s_n = c_s, r_n = c_r + c_count;
-      if (r_n >= c_nb * segs) {
+      int64_t s_n = c_s, r_n = c_r + past;
+      if (r_n >= (c_nb + kDiffSegmentCost) * segs) {
         ++s_n;
         r_n = 0;
       }
@@ -677,7 +698,7 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       }
     } else {
       if (r8 < hg) {
-        const int64_t slot = ((v * 2 + (first ? 0 : 1)) * 2 + map) * p.hg_max + r8;
+        const int64_t slot = ((v * 2 + (c_gpos == b0 ? 0 : 1)) * 2 + map) * p.hg_max + r8;
         float* po = p.part_o32 + slot * (2 * HD) + 4 * g;
 #pragma unroll
         for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(po + 16 * n) = o[n];
@@ -691,7 +712,6 @@ __device__ __forceinline__ void diff_range(const DiffParams& p, const Sched& sc,
       }
     }
     prologue = false;
-    first = false;
     if (!has_next) break;
     // the next piece becomes current: its first PF blocks are in flight, in
     // buffers 0 .. PF-1 (n_pad is a multiple of NBUF)
@@ -773,7 +793,7 @@ void diff_stream_kernel(const DiffParams p) {
       const bool in = s <= last;
       PAL_DEBUG_FLAG(in && keys[k] > max_tokens, kDebugLength);
       const int64_t len = !in || keys[k] < 0 ? 0 : (keys[k] > max_tokens ? max_tokens : keys[k]);
-      vals[k] = ((len + 15) >> 4) * segs;
+      vals[k] = len > 0 ? (((len + 15) >> 4) + kDiffSegmentCost) * segs : 0;
       if (in) {
         lds.len[s] = static_cast<int32_t>(len);
         lds.seq[s] = static_cast<int32_t>(seq[k]);
@@ -847,7 +867,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
   if (h >= min(8, p.group - h0)) return;
   const int head = (seg / p.head_chunks) * p.group + h0 + h;
   const int nc = static_cast<int>(vworker_of(sc, g0 + nb - 1) - e) + 1;
-  const int t0 = vstart(sc, e) >= g0 ? 0 : 1;  // the first piece's partial slot
+  const int t0 = vstart(sc, e) == g0 ? 0 : 1;  // the first piece's partial slot: 0 where the range starts with it
   const int lane = lane_id();
   const int w = wave_id();
   const int rl = lane % kLpr;

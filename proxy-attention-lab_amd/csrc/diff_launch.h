@@ -16,7 +16,7 @@ hipError_t launch_diff_t(const DiffParams& p, hipStream_t stream) {
     if (p.q2seq)
       hipLaunchKernelGGL((diff_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
     else
-      hipLaunchKernelGGL((decode_plan_kernel<HD, TPP>), dim3(1), dim3(kPlanThreads), 0, stream, p);
+      hipLaunchKernelGGL((decode_plan_kernel<HD, TPP, kDiffSegmentCost>), dim3(1), dim3(kPlanThreads), 0, stream, p);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
