@@ -171,14 +171,31 @@ struct DiffTileLds {
   float scl[KV8 ? 8 * kPidChunk : 1];  // fp8: scales of each staged page id, [K1, K2, V1, V2][slot]
   int lim[kDiffMRows + 2 * kPfWaves + 1];
   uint64_t other[kDiffMRows / kWave];  // rows of another sequence than the tile's
-  uint32_t next[2];
+  uint32_t next[4];  // the next item, its claim queue, and its tile's entry in the list
   int tile[8];  // the tile: first row, rows, kv pair, first head, heads, claim queue
+  float lam[16];  // lambdas of the tile's heads
   __attribute__((aligned(16))) float weight[2 * HD];  // what a row is scaled with behind its norm
 };
 
-// Item `item`: head group item % G (G = kv pairs x head chunks) of tile item / G.
+// Entry in the list of an item's tile: {first row, sequence}.
+__device__ __forceinline__ const uint32_t* diff_entry(DiffArgs* p, unsigned item) {
+  const unsigned index = item / (static_cast<unsigned>(p->num_kv_heads) * p->tile_chunks);
+  return p->tiles + 2 * (p->hdr[3] ? index : static_cast<unsigned>(p->hdr[2]) - 1 - index);
+}
+
+// Item of claim n in queue q of a grid of nb workgroups: queue q has items q, q + 8,
+// ..., whose first ceil((nb - q) / 8) are taken by place.
+__device__ __forceinline__ unsigned diff_item_of(uint32_t q, uint32_t n, unsigned nb) {
+  return q + kDiffQueues * (n + (nb + kDiffQueues - 1 - q) / kDiffQueues);
+}
+
+// Item `item`, head group item % G (G = kv pairs x head chunks) of the tile of
+// sequence seq_u that begins at row row0.  Claims the next item behind its last
+// step (while the norm is made; a claim at the tile's start would hand the last
+// items to the workgroups that began first, which have the longest).
 template <int DT, int HD, int TPP, bool KV8>
-__device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTileLds<HD, KV8>& L) {
+__device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row0, uint32_t seq_u,
+                                          DiffTileLds<HD, KV8>& L) {
   constexpr int VD = 2 * HD;
   constexpr int KS = HD / 16;  // QK k-steps of a map; also row tiles of 32 value dims
   constexpr int NQ = 2 * KS;   // QK MFMAs of a step (and PV operands, two MFMAs each)
@@ -193,11 +210,7 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTil
 
   DiffArgs* args = diff_args();
   const unsigned G = static_cast<unsigned>(args->num_kv_heads) * args->tile_chunks;
-  const unsigned index = item / G;
-  const unsigned grp = item - index * G;
-  const uint32_t* entry = args->tiles + 2 * (args->hdr[3] ? index : static_cast<unsigned>(args->hdr[2]) - 1 - index);
-  const int row0 = uniform(static_cast<int>(entry[0]));
-  const uint32_t seq_u = static_cast<uint32_t>(uniform(static_cast<int>(entry[1])));
+  const unsigned grp = item % G;
   const int tile_heads = args->tile_heads;
   const int pair = static_cast<int>(grp / args->tile_chunks);
   const int h0 = static_cast<int>(grp % args->tile_chunks) * tile_heads;
@@ -249,6 +262,7 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTil
       qv[r][kk] = *reinterpret_cast<const u32x4*>(qp + (F8 ? 32 * (kk / 2) + 16 * half + 8 * (kk % 2) : 16 * kk + 8 * half));
   }
   __syncthreads();  // the previous tile is done with every LDS array
+  if (tid < 16) L.lam[tid] = args->lambdas[pair * args->group + h0 + (tid < hg ? tid : 0)];
   if (tid < VD) L.weight[tid] = args->out_scale * (args->norm_weight ? args->norm_weight[tid] : 1.f);
   if (w < kDiffMRows / kWave) {
     const uint64_t m = __ballot(row_seq != seq_u);
@@ -907,9 +921,13 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTil
   // as whole rows.
   DiffArgs* out_args = diff_args();
   const int out_lane = lane_now(), out_col = out_lane & 31, out_half = out_lane >> 5;
+  const bool claims = w == 0 && out_lane == 0 &&
+                      static_cast<unsigned>(out_args->hdr[2]) * out_args->num_kv_heads * out_args->tile_chunks > gridDim.x;
+  uint32_t claimed = 0;
+  if (claims) claimed = atomicAdd(out_args->claim + uniform(L.tile[5]), 1u);
   const float l1 = sum_xor32(l_run[0]), l2 = sum_xor32(l_run[1]);
   const float f1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f;  // (no score above -inf: the map adds nothing)
-  const float f2 = l2 > 0.f || l2 != l2 ? -out_args->lambdas[head] / l2 : 0.f;
+  const float f2 = l2 > 0.f || l2 != l2 ? -L.lam[row_ok ? my_h : 0] / l2 : 0.f;
   float ss[4] = {0.f, 0.f, 0.f, 0.f};
   static_for<KS * 16>([&](auto xc) {
     constexpr int X = decltype(xc)::value;
@@ -919,6 +937,24 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, DiffTil
   if (out_args->norm_weight)
     scale = 1.f / sqrtf(sum_xor32((ss[0] + ss[1]) + (ss[2] + ss[3])) * (1.f / VD) + out_args->norm_eps);
   __syncthreads();  // every wavefront has read the last step
+  if (claims) {
+    DiffArgs* p = diff_args();
+    const unsigned items = static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks;
+    uint32_t q = L.tile[5];
+    unsigned next = diff_item_of(q, claimed, gridDim.x);
+#pragma unroll 1
+    for (int k = 1; k < kDiffQueues && next >= items; ++k) {  // that queue is empty: the next one with an item
+      q = (q + 1) % kDiffQueues;
+      next = diff_item_of(q, atomicAdd(p->claim + q, 1u), gridDim.x);
+    }
+    L.next[0] = next;
+    L.next[1] = q;
+    if (next < items) {
+      const uint32_t* entry = diff_entry(p, next);
+      L.next[2] = entry[0];
+      L.next[3] = entry[1];
+    }
+  }
   constexpr int kCh = VD / 8;  // 16-byte chunks of a row
   auto place_chunk = [](int row, int c) { return (kCh & (kCh - 1)) == 0 ? c ^ (row & (kCh - 1)) : (c + row) % kCh; };
   static_assert(sizeof(L.k) + sizeof(L.v) >= 128 * VD * 2, "the step buffers hold the tile's rows");
@@ -956,33 +992,25 @@ template <int DT, int HD, int TPP, bool KV8>
 __global__ __launch_bounds__(kPfThreads) PAL_DIFF_TILE_KERNEL void diff_tile_kernel(const DiffParams) {
   extern __shared__ __attribute__((aligned(16))) uint8_t tile_lds[];
   DiffTileLds<HD, KV8>& L = *reinterpret_cast<DiffTileLds<HD, KV8>*>(tile_lds);
-  uint32_t queue = blockIdx.x % kDiffQueues;
   unsigned item = blockIdx.x;
-  for (;;) {
-    {
-      DiffArgs* p = diff_args();
-      if (item >= static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks) return;
-    }
-    diff_tile<DT, HD, TPP, KV8>(item, queue, L);
+  uint32_t queue = item % kDiffQueues;
+  {
     DiffArgs* p = diff_args();
-    const unsigned nb = gridDim.x;
+    if (item >= static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks) return;
+  }
+  const uint32_t* entry = diff_entry(diff_args(), item);
+  uint32_t row0 = __builtin_amdgcn_readfirstlane(entry[0]), seq = __builtin_amdgcn_readfirstlane(entry[1]);
+  for (;;) {
+    diff_tile<DT, HD, TPP, KV8>(item, queue, static_cast<int>(row0), seq, L);
+    DiffArgs* p = diff_args();
     const unsigned items = static_cast<unsigned>(p->hdr[2]) * p->num_kv_heads * p->tile_chunks;
-    if (items <= nb) return;
-    // queue q: items q, q + 8, ...; its first ceil((nb - q) / 8) are taken by place
-    auto item_of = [&](uint32_t q, uint32_t n) { return q + kDiffQueues * (n + (nb + kDiffQueues - 1 - q) / kDiffQueues); };
-    if (threadIdx.x == 0) {
-      uint32_t q = L.tile[5];
-      unsigned next = item_of(q, atomicAdd(p->claim + q, 1u));
-      for (int k = 1; k < kDiffQueues && next >= items; ++k) {  // that queue is empty: the next one with an item
-        q = (q + 1) % kDiffQueues;
-        next = item_of(q, atomicAdd(p->claim + q, 1u));
-      }
-      L.next[0] = next;
-      L.next[1] = q;
-    }
+    if (items <= gridDim.x) return;
     __syncthreads();
     item = __builtin_amdgcn_readfirstlane(L.next[0]);
+    if (item >= items) return;
     queue = __builtin_amdgcn_readfirstlane(L.next[1]);
+    row0 = __builtin_amdgcn_readfirstlane(L.next[2]);
+    seq = __builtin_amdgcn_readfirstlane(L.next[3]);
   }
 }
 
