@@ -625,7 +625,7 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
   // of K read in the PV half and all of V in the QK half, the LDS would be
   // asked for its whole rate in the latter, and twice the registers hold
   // operands.
-  constexpr int kAhead = HD == 128 ? 8 : (HD == 96 ? 8 : NQ);
+  constexpr int kAhead = HD == 128 ? (F8 ? 6 : 8) : (HD == 96 ? 8 : NQ);
   Op ka[NQ];
   const int paged_full = !long_pages ? max_lim / kKeys : 0;  // whole steps
   if (nsteps > 0) {
@@ -729,10 +729,16 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
       l_run[r] += p1;
 #pragma unroll
       for (int h = 0; h < NP; ++h) {
-        pp[r][ks][h][i] = F8 ? Dt<DT>::pack2(p0 * vsm[h], p1 * vsm[h]) : Dt<DT>::pack2(p0, p1);
         // held here: code motion would sink the conversion to the MFMA that reads
         // it, which (as inline assembly) must stand two instructions behind it
-        if (i == 3) asm volatile("" : "+v"(pp[r][ks][h]));
+        if constexpr (F8) {
+          uint32_t w = Dt<DT>::pack2(p0 * vsm[h], p1 * vsm[h]);
+          asm volatile("" : "+v"(w));
+          pp[r][ks][h][i] = w;
+        } else {
+          pp[r][ks][h][i] = Dt<DT>::pack2(p0, p1);
+          if (i == 3) asm volatile("" : "+v"(pp[r][ks][h]));
+        }
       }
     };
     // the operand reads that go out with MFMA n of the step's 3 NQ
@@ -752,7 +758,11 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
         }
       });
     };
-    auto convert_v = [&](int m, u32x2 c) {  // fp8: operand m from its codes
+    auto convert_k = [&](auto c) {  // fp8: an operand from its codes
+      if constexpr (F8) return fp8x8_exact<DT>(c);
+      else return c;
+    };
+    auto convert_v = [&](int m, auto c) {  // fp8: operand m from its codes
       if constexpr (kSplitScale) {
         const float e = vse[(m % KS) / (KS / 2)];
         u32x4 r;
@@ -764,14 +774,42 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
         }
         return r;
       } else {
-        return fp8x8_exact<DT>(c);
+        return convert_k(c);
       }
     };
+    // fp8: operands are converted a chunk ahead of their MFMA, before the chunk's
+    // other work: an MFMA stands two wait states or more behind a conversion (with
+    // conversions right before their MFMA and the waits filled with s_nop, a step
+    // of HD 128 took 1.62 us, now 1.55)
+    u32x4 op[2];
+    auto converted = [&](int i) {
+      asm volatile("" : "+v"(op[i]));
+      sched_fence();
+    };
+    auto two_waits = [] { asm volatile("s_nop 1"); };
+    if constexpr (F8 && kMode != kLast) {
+      op[0] = convert_k(ka[0]);
+      converted(0);
+      two_waits();
+    }
     // ---- QK MFMAs of step st + 1; exponentials of the first 16 keys' pairs
     static_for<NQ>([&](auto cc) {
       constexpr int c = decltype(cc)::value;
-      if constexpr (kMode != kLast) qk(cc, s_next, ka[c]);
+      if constexpr (kMode != kLast) {
+        if constexpr (F8) diff_qk<DT, false, (c < 2)>(s_next[c % 2], op[c % 2], qv[c % 2][c / 2]);
+        else qk(cc, s_next, ka[c]);
+      }
       reads_at(cc);
+      if constexpr (F8) {
+        if constexpr (c + 1 == NQ) {
+          op[0] = convert_v(0, va[0]);
+          converted(0);
+        } else if constexpr (kMode != kLast) {
+          op[(c + 1) % 2] = convert_k(ka[c + 1]);
+          converted((c + 1) % 2);
+        }
+        if constexpr (c * 8 / NQ == (c + 1) * 8 / NQ && (c == 0 || (c - 1) * 8 / NQ == c * 8 / NQ)) two_waits();
+      }
 #pragma unroll
       for (int q = c * 8 / NQ; q < (c + 1) * 8 / NQ; ++q) pair_exp(q);
       if constexpr (c > 0) {
@@ -799,7 +837,6 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
       sc[1] = F8 ? score_scale(1, st + 1) : sc[0];
     }
     constexpr int NPV = 2 * NQ;  // chunk c: operand c / 2, map c % 2
-    u32x4 vop;
     static_for<NPV>([&](auto cc) {
       constexpr int c = decltype(cc)::value;
       constexpr int m = c / 2, r = c % 2, ks = m / KS, t = m % KS;
@@ -814,20 +851,23 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
         }
       }
       if constexpr (F8) {
-        if constexpr (r == 0) {
-          vop = convert_v(m, va[m]);
-          asm volatile("s_nop 1" : "+v"(vop));
-        }
-        diff_mma<DT, false, r * KS + t>(vop, pp[r][ks][t / (KS / 2)]);
+        diff_mma<DT, false, r * KS + t>(op[m % 2], pp[r][ks][t / (KS / 2)]);
       } else {
         diff_mma<DT, true, r * KS + t>(va[m], pp[r][ks][0]);
       }
       reads_at(std::integral_constant<int, NQ + c>{});
+      if constexpr (F8 && r == 1 && m + 1 < NQ) {
+        op[(m + 1) % 2] = convert_v(m + 1, va[m + 1]);
+        converted((m + 1) % 2);
+        if constexpr (kMode == kLast) two_waits();
+      }
       if constexpr (c == 0) {
         static_for<8>([&](auto qq) {
           constexpr int q = decltype(qq)::value;
           if constexpr (q >= (NQ - 1) * 8 / NQ) pair_pack(q);
         });
+        sched_fence();
+        two_waits();  // the next MFMA may multiply that pair
       }
       // first half: exponentials of the other 16 keys
       if constexpr (c < NQ) {
@@ -859,6 +899,7 @@ __device__ __forceinline__ void diff_tile(unsigned item, uint32_t queue, int row
           if constexpr (q >= (NQ - 1) * 8 / NQ) pair_pack(8 + q);
         });
         sched_fence();
+        if constexpr (kMode == kLast) two_waits();
       }
     });
     if constexpr (kMode == kLast) {
