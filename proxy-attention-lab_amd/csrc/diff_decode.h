@@ -843,7 +843,9 @@ void diff_stream_kernel(const DiffParams p) {
 // Joins the pieces of split segments: workgroup (v, h) takes head h of the
 // segment in list slot v, whose first piece is worker v's, further pieces the
 // first ones of workers v + 1, v + 2, ...  A wavefront takes every fourth piece
-// (times the rows one 16-byte load per lane covers), all maxima first:
+// (times the rows one 16-byte load per lane covers), all maxima first (the first
+// rows load beside them, as the lambda and the weight do: the kernel's time is
+// its chain of loads):
 //   O_m = sum_c 2^(M_c - M) O_c,  l_m = sum_c 2^(M_c - M) l_c
 // the wavefronts' sums meet in LDS, and the first finishes the row.
 template <int DT, int HD>
@@ -875,6 +877,25 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
   const bool dl = 4 * rl < D;
   auto row_of = [&](int c, int map) { return (((e + c) * 2 + (c == 0 ? t0 : 0)) * 2 + map) * p.hg_max + h; };
 
+  f32x2 ml[kBatch][2];
+  f32x4 o[kBatch][2];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * kDiffWaves * kRows + rg;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int64_t r = row_of(c < nc ? c : nc - 1, m);  // (past the last: read again, weight 0)
+        ml[u][m] = *reinterpret_cast<const f32x2*>(p.part_ml + r * 2);
+        o[u][m] = *reinterpret_cast<const f32x4*>(p.part_o32 + r * D + (dl ? 4 * rl : 0));
+      }
+    }
+  };
+  constexpr int kStep = kDiffWaves * kRows * kBatch;
+  const float lam = p.lambdas[head];
+  f32x4 weight = {1.f, 1.f, 1.f, 1.f};
+  if (p.norm_weight && dl) weight = *reinterpret_cast<const f32x4*>(p.norm_weight + 4 * rl);
+  load(w * kRows);
   float big[2] = {-INFINITY, -INFINITY};
   for (int c = lane; c < nc; c += kWave) {
 #pragma unroll
@@ -889,19 +910,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
     ref[m] = big[m] == -INFINITY ? 0.f : big[m];
     acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (int c0 = w * kRows; c0 < nc; c0 += kDiffWaves * kRows * kBatch) {
-    f32x2 ml[kBatch][2];
-    f32x4 o[kBatch][2];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int c = c0 + u * kDiffWaves * kRows + rg;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const int64_t r = row_of(c < nc ? c : nc - 1, m);  // (past the last: read again, weight 0)
-        ml[u][m] = *reinterpret_cast<const f32x2*>(p.part_ml + r * 2);
-        o[u][m] = *reinterpret_cast<const f32x4*>(p.part_o32 + r * D + (dl ? 4 * rl : 0));
-      }
-    }
+  for (int c0 = w * kRows; c0 < nc; c0 += kStep) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (c0 + u * kDiffWaves * kRows + rg < nc) {
@@ -913,6 +922,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
         }
       }
     }
+    if (c0 + kStep < nc) load(c0 + kStep);
   }
 #pragma unroll
   for (int off = kLpr; off < kWave; off <<= 1) {
@@ -944,7 +954,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
       om += *reinterpret_cast<const f32x4*>(&sum_lds[u][m][dl ? 4 * rl : 0]);
     }
     const float inv = lm > 0.f || lm != lm ? 1.f / lm : 0.f;
-    x += om * (m ? -p.lambdas[head] * inv : inv);
+    x += om * (m ? -lam * inv : inv);
   }
   float scale = p.out_scale;
   if (p.norm_weight) {
@@ -955,7 +965,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_merge_kernel(const DiffPara
   }
   if (rg == 0 && dl) {
     f32x4 y = x * scale;
-    if (p.norm_weight) y *= *reinterpret_cast<const f32x4*>(p.norm_weight + 4 * rl);
+    if (p.norm_weight) y *= weight;
     *reinterpret_cast<u32x2*>(p.out + (row * (p.num_q_heads / 2) + head) * D + 4 * rl) =
         u32x2{Dt<DT>::pack2(y[0], y[1]), Dt<DT>::pack2(y[2], y[3])};
   }

@@ -22,6 +22,7 @@ from __future__ import annotations
 import collections
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -785,6 +786,13 @@ def _on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+@functools.lru_cache(maxsize=256)
+def _differential_workspace(device: int, code: int, kv_code: int, rows: int, hq: int, hkv: int, hd: int,
+                            tpp: int) -> int:
+    """Workspace bytes of a call on the current device, which `device` names (0: refused by the call itself)."""
+    return _lib.lib().pal_paged_differential_attention_workspace_size(code, kv_code, rows, hq, hkv, hd, tpp)
+
+
 def _differential(op: str, queries, k_pool, v_pool, page_table, lengths, q2s, offsets, lambdas, stream, norm_weight,
                   norm_eps, out_scale, k_scales, v_scales) -> torch.Tensor:
     """Validation, allocation and launch shared by the differential attention
@@ -832,7 +840,9 @@ def _differential(op: str, queries, k_pool, v_pool, page_table, lengths, q2s, of
             out = torch.empty((rows, hq // 2, 2 * hd), dtype=queries.dtype, device=device)
             # a workspace of the call's own (it needs no initial contents): calls captured
             # into different graphs share nothing
-            nbytes = L.pal_paged_differential_attention_workspace_size(code, kv_code, rows, hq, hkv, hd, tpp)
+            nbytes = _differential_workspace(device.index, code, kv_code, rows, hq, hkv, hd, tpp)
+            if nbytes == 0:  # refused below; not kept, the device may have been at fault
+                _differential_workspace.cache_clear()
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
             entry = L.pal_paged_differential_attention_decode if q2s is None else L.pal_paged_differential_attention
             status = entry(
