@@ -323,26 +323,62 @@ __device__ __forceinline__ int rope_axis(const FillParams& p, int f) {
   }
   return (f >= p.rope_section_end[0]) + (f >= p.rope_section_end[1]) + (f >= p.rope_section_end[2]);
 }
-// Do all positions of token t have a row in the table?
+// Do all positions of token t have a row in the table?  (Axes past the last load
+// that again: four loads in flight together.)
 __device__ __forceinline__ bool rope_axes_ok(const FillParams& p, int64_t t) {
+  int pos[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) pos[a] = p.rope_pos[min(a, p.rope_axes - 1) * p.num_tokens + t];
   bool ok = true;
-  for (int a = 0; a < p.rope_axes; ++a) {
-    const int pos = p.rope_pos[a * p.num_tokens + t];
-    ok = ok && pos >= 0 && pos < p.cos_sin_rows;
-  }
+#pragma unroll
+  for (int a = 0; a < 4; ++a) ok = ok && pos[a] >= 0 && pos[a] < p.cos_sin_rows;
   return ok;
 }
 // Gathers the cos/sin rows of the window's tokens into LDS (a position without a
-// row takes row 0: such a token is not rotated).
+// row takes row 0: such a token is not rotated).  Each element is two dependent
+// loads: a thread's are in flight four at a time, indexes carried along (12 prompts
+// of 512-2,048 tokens, 8 + 32 heads of 128: 103 us one at a time with their
+// divisions, 93 so).  By the threads from kFirst on: beside K and V the first
+// wavefront looks up the destinations meanwhile (91 us).
+template <int kFirst>
 __device__ __forceinline__ void gather_rope_rows(const FillParams& p, int64_t t0, int nwin, float* rows) {
+  constexpr int kBatch = 4;
+  constexpr int kCount = kThreads - kFirst;
+  const int tid = static_cast<int>(threadIdx.x) - kFirst;
+  if (tid < 0) return;
   const int half = p.rotary_dim / 2;
-  for (int it = threadIdx.x; it < nwin * half; it += kThreads) {
-    const int i = it / half;
-    const int f = it - i * half;
-    const int pos = p.rope_pos[rope_axis(p, f) * p.num_tokens + t0 + i];
-    const float* cs = p.cos_sin + (pos >= 0 && pos < p.cos_sin_rows ? static_cast<int64_t>(pos) * p.rotary_dim : 0);
-    rows[i * p.rotary_dim + f] = cs[f];
-    rows[i * p.rotary_dim + half + f] = cs[half + f];
+  const int total = nwin * half;
+  const int di = kCount / half, df = kCount - di * half;
+  int i = tid / half, f = tid - i * half;
+#pragma unroll 1
+  for (int it = tid; it < total; it += kBatch * kCount) {
+    int pos[kBatch], token[kBatch], freq[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      token[k] = it + k * kCount < total ? i : -1;
+      freq[k] = f;
+      pos[k] = p.rope_pos[rope_axis(p, f) * p.num_tokens + t0 + (token[k] < 0 ? 0 : i)];
+      i += di;
+      f += df;
+      if (f >= half) {
+        f -= half;
+        ++i;
+      }
+    }
+    float c[kBatch], sn[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const bool ok = pos[k] >= 0 && pos[k] < p.cos_sin_rows;
+      const float* cs = p.cos_sin + (ok ? static_cast<int64_t>(pos[k]) * p.rotary_dim : 0) + freq[k];
+      c[k] = cs[0];
+      sn[k] = cs[half];
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (token[k] < 0) continue;
+      rows[token[k] * p.rotary_dim + freq[k]] = c[k];
+      rows[token[k] * p.rotary_dim + half + freq[k]] = sn[k];
+    }
   }
 }
 
@@ -387,19 +423,38 @@ __device__ __forceinline__ void rotate_queries_axes(const FillParams& p, int64_t
   const int64_t q_row = static_cast<int64_t>(p.num_q_heads) * hd;
   // element offset of unit u's first (and partner) piece in its head
   auto dim0 = [&](int u) { return u < pairs ? kVal * u : kVal * (u + pairs); };
+  // item it: unit u of head h0 + hq of token i, carried along from item to item
+  const int d_th = kThreads / units, du = kThreads - d_th * units;
+  const int di = d_th / nh, dh = d_th - di * nh;
+  const int th0 = static_cast<int>(threadIdx.x) / units;
+  int u = static_cast<int>(threadIdx.x) - th0 * units;
+  int i = th0 / nh, hq = th0 - i * nh;
 #pragma unroll 1
   for (int base = 0; base < n_items; base += kItems * kThreads) {
     u32x4 a[kItems], b[kItems];
+    int unit[kItems], token[kItems];
+    int64_t at[kItems];
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const int it = base + static_cast<int>(threadIdx.x) + k * kThreads;
+      unit[k] = u;
+      token[k] = i;
+      at[k] = (t0 + i) * q_row + static_cast<int64_t>(h0 + hq) * hd + dim0(u);
       if (it < n_items) {
-        const int th = it / units, u = it - th * units;
-        const int i = th / nh;
-        const int64_t elem = (t0 + i) * q_row + static_cast<int64_t>(h0 + th - i * nh) * hd + dim0(u);
-        const uint8_t* src = static_cast<const uint8_t*>(p.q_in) + elem * kSrcBytes;
+        const uint8_t* src = static_cast<const uint8_t*>(p.q_in) + at[k] * kSrcBytes;
         a[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src));
         if (u < pairs) b[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + half * kSrcBytes));
+      }
+      u += du;
+      hq += dh;
+      i += di;
+      if (u >= units) {
+        u -= units;
+        ++hq;
+      }
+      if (hq >= nh) {
+        hq -= nh;
+        ++i;
       }
     }
     if (base == 0) __syncthreads();  // the gathered rows are complete
@@ -407,9 +462,8 @@ __device__ __forceinline__ void rotate_queries_axes(const FillParams& p, int64_t
     for (int k = 0; k < kItems; ++k) {
       const int it = base + static_cast<int>(threadIdx.x) + k * kThreads;
       if (it >= n_items) continue;
-      const int th = it / units, u = it - th * units;
-      const int i = th / nh;
-      const int64_t elem = (t0 + i) * q_row + static_cast<int64_t>(h0 + th - i * nh) * hd + dim0(u);
+      const int u = unit[k], i = token[k];
+      const int64_t elem = at[k];
       const float* cs = rows + i * rot;
       float x[kVal], y[kVal], xo[kVal], yo[kVal];
       piece_to_f32<SRC>(a[k], x);
@@ -481,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
     if (static_cast<int>(blockIdx.y) >= p.num_kv_heads) {
       const int h0 = (static_cast<int>(blockIdx.y) - p.num_kv_heads) * kAxesQueryHeads;
       if (tid < nwin) kind_lds[tid] = rope_axes_ok(p, t0 + tid);
-      gather_rope_rows(p, t0, nwin, rope_rows);
+      gather_rope_rows<0>(p, t0, nwin, rope_rows);
       rotate_queries_axes<SRC, 4>(p, t0, nwin, h0, min(kAxesQueryHeads, p.num_q_heads - h0), rope_rows, kind_lds);
       return;
     }
@@ -671,7 +725,7 @@ __global__ __launch_bounds__(kThreads) void fill_kv_pages_kernel(const FillParam
     ks_lds[tid] = ks;
     vs_lds[tid] = vs;
   }
-  if constexpr (kMode == kRopeAxes) gather_rope_rows(p, t0, nwin, rope_rows);
+  if constexpr (kMode == kRopeAxes) gather_rope_rows<kWave>(p, t0, nwin, rope_rows);
   __syncthreads();
   // the cos/sin row of window token i
   auto rope_row = [&](int i) {
