@@ -352,7 +352,8 @@ int pal_paged_attention_fp8(const void* queries, const void* k_pool, const void*
  * lambdas: fp32 [num_q_heads / 2]; norm_weight: fp32 [2 head_dim], shared by the
  * heads, or NULL.  out: [rows, num_q_heads / 2, 2 head_dim] in dtype.  Sums,
  * softmax statistics and both maps' outputs are held in fp32 until y is rounded;
- * the probabilities are rounded to dtype for their product with the values.
+ * the probabilities are rounded to 16 bits for their product with the values
+ * (rows alone in their run of rows: to two terms of 16 bits).
  * Rows without a visible key are zeros.  num_kv_heads even; kv_dtype dtype or
  * fp8 (with k_scales and v_scales); head_dim 32, 64, 96 or 128 (fp8: 64, 128);
  * tokens_per_page 16 or 32.  All pointers but lambdas, the index arrays and the
