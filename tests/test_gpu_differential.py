@@ -414,6 +414,37 @@ def test_graphs_share_nothing():
             assert np.array_equal(host_bits(o), w), f"replay {r}"
 
 
+def test_graph_replays_plan_anew():
+    """A captured mixed batch whose lengths, limits and rows' sequences change between replays: lone rows, tiles and
+    their order are found at every replay, on both sides of the rows that are planned in the stream kernel."""
+    rng = np.random.default_rng(34)
+    for rows in (700, 1500):
+        lens = rng.integers(1, 90, 300).tolist()
+        d = chunk_case(34, lens, [(30, rows - 500), (0, 200)], 8, 4, 32, 16, "bf16")
+        seqs = len(d.case.seq_lens)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            d.run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        announce(f"graph capture: {rows} rows")
+        with torch.cuda.graph(g, stream=side):
+            out = d.run()
+        for r in range(4):
+            n = int(d.off.shape[0])
+            q2s = np.sort(rng.integers(0, seqs, n)) if r % 2 else np.repeat(rng.permutation(seqs), -(-n // seqs))[:n]
+            d.dev["q2s"].copy_(dev_index(q2s.astype(np.uint32), torch.uint32))
+            d.dev["off"].copy_(dev_index(rng.integers(-3, 300, n).astype(np.int32)))
+            d.dev["lens"].copy_(dev_index((d.case.seq_lens * rng.integers(0, 2, seqs)).astype(np.int32)))
+            want = host_bits(d.run())
+            torch.cuda.synchronize()
+            announce(f"graph replay {r} of {rows} rows")
+            g.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(host_bits(out), want), f"replay {r} of {rows} rows"
+
+
 def test_refusals():
     d = decode_case(40, [40, 20], 8, 4, 64, 16, "bf16")
     x = d.dev
